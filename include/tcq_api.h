@@ -246,6 +246,15 @@ int tcq_post_add_norm_pre(const void* acc, int acc_dtype, int lda, int col0, con
                           const float* bias, const void* x, void* xout, const void* w, float eps, const int8_t* su, int8_t* q,
                           int32_t* q4, int ldq, float* scale, int M, int N, tcq_stream_t stream);
 
+/* Residual addition, RMSNorm and INT8 rows of the next product in one pass, without a rotation (what tcq_quantize_rows after a norm
+ * gives tcq_gemm_i8): h = x + r rounded to dtype (r NULL: h = x), n = h / sqrt(mean(h^2) + eps) * (offset + w) (offset 1: Gemma's weights,
+ * 0: plain ones), scale[t] = max|n| / 127 (1 for a row of zeros), q = rint(n / scale). x, r, xout (M, K) of dtype F32, BF16 or F16 with row
+ * strides in elements, w (K,) of dtype; xout (NULL: not stored) may be x or r; q (M, K) int8 contiguous and / or q4 / ldq as tcq_pre.
+ * FP32 sums; n itself is not rounded before its codes. A row with a value that is not finite has scale NaN. K <= 32768. No
+ * reference counterpart: the reference leaves the policy's norms to PyTorch. */
+int tcq_add_norm_quantize(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, float eps, float offset, int dtype, void* xout,
+                          int64_t ldo, int8_t* q, int32_t* q4, int ldq, float* scale, int M, int K, tcq_stream_t stream);
+
 /* Attention of H <= 8 query heads over one shared key / value head of dim D = 256 (multi-query), BF16 in and out, FP32
  * arithmetic. q (M, H * D); keys / values = the P cache rows (k_cache, v_cache (P, D); NULL when P = 0) followed by this
  * call's M rows (k_new, v_new (M, D)); query t sees key j iff causal_offset < 0 or j <= causal_offset + t. Scores
@@ -288,6 +297,56 @@ int tcq_attend_q4_static(const void* q, const void* k_cache, const void* v_cache
                          int H, int D, int causal_offset, void* o, const int8_t* su, int8_t* q8, int32_t* q4, int ldq, float* scale,
                          tcq_stream_t stream);
 size_t tcq_attend_static_floats(void);
+
+/* ------------------------------------------------------------------------- rotary positions and the 8-bit cache */
+
+/* Rotary positions with A axes (time, height, width; A = 1: the usual ones) on M tokens of Hq query and Hk key heads (Hk = 0: one
+ * tensor only), D values each: pair i of the first R of a head's values turns by a = pos[axis[i]] * freq[i], (x1, x2) ->
+ * (x1 cos a - x2 sin a, x2 cos a + x1 sin a), or by -a with inverse != 0 (the gradient of the rotation, and the way back). The pairs
+ * are (i, i + R / 2), or (2 i, 2 i + 1) with adjacent != 0; the values from R on are copied. x, out: dtype F32, BF16 or F16, token and
+ * head strides in elements, a head's values contiguous; out may be x (in place). pos: A x M int32 (pos64 = 0) or int64, strides in
+ * elements; freq (R / 2,) FP64, radians per position; axis (R / 2,) int32 (NULL: all 0; outside 0 .. A - 1: the pair is not turned).
+ * Angles are reduced in FP64. No reference counterpart: the reference leaves positions to PyTorch. */
+int tcq_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head, int Hq, const void* k,
+                  int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok, int64_t ko_head, int Hk, int dtype, const void* pos, int pos64,
+                  int64_t pos_axis, int64_t pos_tok, const double* freq, const int32_t* axis, int A, int M, int D, int R, int adjacent,
+                  int inverse, tcq_stream_t stream);
+
+/* A key / value cache in 8 bits: B sequences, H KV heads of D = 64, 128 or 256, nblk blocks of TCQ_KV8_BLOCK tokens each. A block of a
+ * head has one FP32 scale for its keys and one for its values, scale = max|x| / 127 over the rows that it holds (1 for zeros), codes
+ * rint(x / scale). Infinities count as the block's largest code and NaN as 0: 8 bits have neither.
+ *   k8 (B, H, nblk, 4, D / 16, 16, 16) int8 = (token / 16, dim / 16, token % 16, dim % 16)
+ *   v8 (B, H, nblk, D / 16, 4, 16, 16) int8 = (dim / 16, token % 16 / 4, dim % 16, token / 16 * 4 + token % 4)
+ *   scale (B, H, nblk, 2) FP32 (keys, values); tail (B, H, 2, 2, 64, D) of the rows' type = (block % 2, keys | values, token, dim):
+ *   the 16-bit rows of the newest two blocks.
+ * All 16-byte aligned. No reference counterpart (the reference leaves the cache to PyTorch). */
+#define TCQ_KV8_BLOCK 64
+
+/* Rows into the cache: sequence b's rows cu[b] .. cu[b + 1] - 1 (cu NULL: most rows each) of k, v (rows, H, D), BF16 or F16, token and
+ * head strides in elements, go to positions start[b], start[b] + 1, ... What a sequence held from start[b] on is gone; the rows
+ * before it in start[b]'s block come from the tail, so start[b] lies at most one whole block before the newest block written
+ * (an append that ended at start[b], or one that is taken back by up to 64 rows). Every touched block is quantized anew from its 16-bit
+ * rows, so a block's codes depend on its rows alone. Rows past the capacity, past `most` of a sequence or past `rows` are dropped;
+ * a sequence without new rows is left as it is. */
+int tcq_kv8_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int dtype, const int32_t* cu,
+                   const int32_t* start, int rows, int most, int B, int H, int D, int nblk, int8_t* k8, int8_t* v8, float* scale, void* tail,
+                   tcq_stream_t stream);
+/* Rows out of the cache: k, v (B, n, H, D) of dtype F32, BF16 or F16, row i of sequence b = code * scale of position first[b] + i, zeros
+ * from lens[b] on. */
+int tcq_kv8_read(const int8_t* k8, const int8_t* v8, const float* scale, const int32_t* first, const int32_t* lens, int n, int B, int H, int D,
+                 int nblk, void* k, void* v, int dtype, tcq_stream_t stream);
+/* Attention over the cache: o = softmax(score_scale q k^T) v, query head i over KV head i / (Hq / Hk), sequence b's rows cu[b] ..
+ * cu[b + 1] - 1 (cu NULL: most rows each) of q (rows, Hq, D; BF16 or F16, strides in elements) over its first lens[b] positions; with
+ * causal, row i of n sees positions j <= lens[b] - n + i. o (rows, Hq, D) contiguous, of q's type. A row that sees nothing is zeros; a query
+ * row with a value that is not finite is NaN; rows of no sequence are left as they were. keys: about the most positions that a
+ * sequence has (it sets how far the work is split, never the result's meaning). part: workspace of tcq_kv8_attend_floats(...) floats,
+ * 16-byte aligned (NULL where that is 0), not shared by calls that overlap. Scores from the query as 16-bit integers (within 2^-16 of the
+ * row's largest value) and the probabilities as 16-bit integers of their block's maximum, exact int32 products with the codes, FP32
+ * maximum, sum and outputs. */
+int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, const int32_t* lens, int rows, int most, int B,
+                   int Hq, int Hk, int D, int nblk, const int8_t* k8, const int8_t* v8, const float* scale, int causal, float score_scale,
+                   int keys, float* part, void* o, tcq_stream_t stream);
+int64_t tcq_kv8_attend_floats(int rows, int most, int B, int Hq, int Hk, int D, int keys);
 
 /* -------------------------------------------------------------------------------------------------------- products */
 

@@ -84,8 +84,14 @@ SIGNATURES = {
     'tcq_gemm_w8_pro': [_P, _I, _P, _I, _I, _I, _P],
     'tcq_attend_parts': [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P],
     'tcq_attend_post_parts': [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P],
+    'tcq_add_norm_quantize': [_P, _L, _P, _L, _P, _F, _F, _I, _P, _L, _P, _P, _I, _P, _I, _I, _P],
+    'tcq_rope_axes': [_P, _L, _L, _P, _L, _L, _I, _P, _L, _L, _P, _L, _L, _I, _I, _P, _I, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    'tcq_kv8_append': [_P, _L, _L, _P, _L, _L, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P],
+    'tcq_kv8_read': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P],
+    'tcq_kv8_attend': [_P, _L, _L, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _I, _F, _I, _P, _P, _P],
+    'tcq_kv8_attend_floats': [_I, _I, _I, _I, _I, _I, _I],
 }
-_RESTYPE = {'tcq_version': ctypes.c_char_p, 'tcq_repack_words': _L, 'tcq_attend_static_floats': ctypes.c_size_t}
+_RESTYPE = {'tcq_version': ctypes.c_char_p, 'tcq_repack_words': _L, 'tcq_kv8_attend_floats': _L, 'tcq_attend_static_floats': ctypes.c_size_t}
 
 MAX_SEGS = 4
 

@@ -2,7 +2,9 @@
 stream. Names and argument meaning follow the reference's launch helpers (deploy/tcq_kernels/kernels.py:572-696); the
 functions added here (rht, pre_h16, quantize_rows, repack, decode_f16, gemv_f16, ...) have no reference counterpart and say so.
 """
+import collections
 import ctypes
+import math
 
 import torch
 
@@ -264,6 +266,222 @@ def post_add_norm_pre(acc, s, rs, sv, bias, x, xout, w=None, eps=0.0, su=None, q
     call('tcq_post_add_norm_pre', ptr(acc), adt, lda, col0, ptr(s), ptr(rs), ptr(sv), ptr(bias), ptr(x), ptr(xout), ptr(w),
          float(eps), ptr(su), ptr(q), ptr(q4), _ldq(q4), ptr(scale), M, N, stream())
     return xout
+
+
+def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offset=1.0):
+    """h = x + r (r None: x), rounded to x's type and stored in xout where that is given (it may be x or r), then INT8 rows of
+    RMSNorm(h) * (offset + w): q (M, K) int8 and / or q4 (as in pre), scale (M,) FP32, what gemm_i8 takes. x, r, xout (M, K) BF16 / FP16
+    / FP32 with contiguous rows of any stride, w (K,) of that type; offset 1: Gemma's weights, 0: plain ones."""
+    M, K = x.shape
+    d = _dt(x, (0, 1, 2), 'add_norm_quantize x')
+    for t in (r, xout):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.stride(1) != 1 and K > 1):
+            raise ValueError(f'add_norm_quantize: r and xout must be ({M}, {K}) {x.dtype} with contiguous rows')
+    if w.dtype != x.dtype or w.numel() != K or (x.stride(1) != 1 and K > 1):
+        raise ValueError(f'add_norm_quantize: w must be ({K},) {x.dtype}, the rows of x contiguous')
+    if scale is None or scale.dtype != torch.float32 or scale.numel() != M:
+        raise ValueError(f'add_norm_quantize: scale must be ({M},) float32')
+    if q is None and q4 is None:
+        raise ValueError('add_norm_quantize: q and / or q4')
+    if q is not None and (q.dtype != torch.int8 or q.shape != x.shape):
+        raise ValueError(f'add_norm_quantize: q must be ({M}, {K}) int8')
+    _q4_holds(q4, M, K, 'add_norm_quantize')
+    _contig(w, q, q4, scale)
+    _one_device('add_norm_quantize', x, r, w, q, q4, scale, xout)
+    if M == 0:
+        return
+    call('tcq_add_norm_quantize', ptr(x), x.stride(0), ptr(r), 0 if r is None else r.stride(0), ptr(w), float(eps), float(offset), d,
+         ptr(xout), 0 if xout is None else xout.stride(0), ptr(q), ptr(q4), _ldq(q4), ptr(scale), M, K, stream())
+
+
+def _q4_holds(q4, M, K, what):
+    """Whether a q4 output (word layout or token blocks) is one of M tokens of K columns."""
+    if q4 is None:
+        return
+    if q4.dim() == 4:
+        ok = q4.dtype == torch.int8 and tuple(q4.shape) == ((M + 15) // 16, K // 16, 16, 16) and K % 16 == 0
+    else:
+        ok = q4.dtype == torch.int32 and q4.dim() == 2 and 4 * q4.shape[0] == K and q4.shape[1] >= M
+    if not ok:
+        raise ValueError(f'{what}: q4 {tuple(q4.shape)} {q4.dtype} does not hold {M} tokens of {K} columns')
+
+
+def _one_device(what, *ts):
+    """The tensors of a call are on the current device: its stream is the one that the kernels run on."""
+    at = None
+    for t in ts:
+        if t is not None:
+            if not t.is_cuda:
+                raise _lib.TcqError(f'{what}: libtcq takes device tensors only (got a CPU tensor)')
+            at = torch.cuda.current_device() if at is None else at
+            if t.get_device() != at:
+                raise ValueError(f'{what}: a tensor is on {t.device}, the current device is cuda:{at}')
+
+
+# --------------------------------------------------------------------------------------- rotary positions, the 8-bit cache
+def rope_frequencies(R, theta=10000.0, sections=None, interleaved=False, device=None):
+    """(freq, axis) of rope_axes for R rotated values of a head: freq[i] = theta^(-2 i / R) (float64), and the axis of every pair:
+    sections (pairs per axis, R / 2 in all) one after the other, or interleaved (axis i % A for as long as the axis has pairs left, the
+    first axis after that); None: one axis."""
+    half = R // 2
+    freq = torch.tensor([float(theta) ** (-i / half) for i in range(half)], dtype=torch.float64, device=device)
+    if sections is None:
+        return freq, torch.zeros(half, dtype=torch.int32, device=device)
+    if sum(sections) != half or R % 2:
+        raise ValueError(f'rope_frequencies: the sections {tuple(sections)} must add up to {half} pairs')
+    A = len(sections)
+    if interleaved:
+        axis = [i % A if i // A < sections[i % A] else 0 for i in range(half)]
+    else:
+        axis = [a for a, n in enumerate(sections) for _ in range(n)]
+    return freq, torch.tensor(axis, dtype=torch.int32, device=device)
+
+
+def _heads(t, what, D=None):
+    if t.dim() != 3 or t.stride(2) != 1 or (D is not None and t.shape[2] != D):
+        raise ValueError(f'{what} must be (tokens, heads, {D or "D"}) with contiguous values, got {tuple(t.shape)}')
+
+
+def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False, inverse=False):
+    """Rotary positions with one or several axes (tcq_rope_axes) of q (M, Hq, D) and k (M, Hk, D) or None, BF16 / FP16 / FP32, any token
+    and head strides (views into a q | k | v row). pos (A, M) or (M,) int32 / int64; freq (R / 2,) float64 and axis (R / 2,) int32 as
+    rope_frequencies makes them, the R first values of a head turn. Outputs None: in place. adjacent: pairs (2 i, 2 i + 1) instead of
+    (i, i + R / 2). inverse: turns back, which is also the gradient."""
+    _heads(q, 'rope_axes q')
+    M, Hq, D = q.shape
+    q_out = q if q_out is None else q_out
+    d = _dt(q, (0, 1, 2), 'rope_axes q')
+    pairs = [(q, q_out)]
+    if k is not None:
+        k_out = k if k_out is None else k_out
+        _heads(k, 'rope_axes k', D)
+        pairs.append((k, k_out))
+    elif k_out is not None:
+        raise ValueError('rope_axes: k_out without k')
+    for x, y in pairs:
+        _heads(y, 'rope_axes outputs', D)
+        if x.shape[0] != M or y.shape != x.shape or x.dtype != q.dtype or y.dtype != q.dtype:
+            raise ValueError('rope_axes: q, k and their outputs must have the same tokens, head size and type')
+    pos = pos[None] if pos.dim() == 1 else pos
+    A, R = pos.shape[0], 2 * freq.numel()
+    if pos.dim() != 2 or pos.shape[1] != M or pos.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f'rope_axes: pos must be (axes, {M}) int32 or int64, got {tuple(pos.shape)} {pos.dtype}')
+    if freq.dtype != torch.float64 or not 0 < R <= D or (axis is not None and (axis.dtype != torch.int32 or axis.numel() != R // 2)):
+        raise ValueError(f'rope_axes: freq must be float64 of at most {D // 2} pairs and axis int32 of as many')
+    _contig(freq, axis)
+    _one_device('rope_axes', q, k, pos, freq, axis, q_out, k_out)
+    if M == 0:
+        return q_out, k_out
+    ks = (None, 0, 0, None, 0, 0, 0) if k is None else (ptr(k), k.stride(0), k.stride(1), ptr(k_out), k_out.stride(0), k_out.stride(1), k.shape[1])
+    call('tcq_rope_axes', ptr(q), q.stride(0), q.stride(1), ptr(q_out), q_out.stride(0), q_out.stride(1), Hq, *ks, d, ptr(pos),
+         int(pos.dtype == torch.int64), pos.stride(0), pos.stride(1), ptr(freq), ptr(axis), A, M, D, R, int(adjacent), int(inverse), stream())
+    return q_out, k_out
+
+
+# A cache of one attention layer in 8 bits (include/tcq_api.h): k8 (B, H, blocks, 4, D / 16, 16, 16) and v8 (B, H, blocks, D / 16, 4, 16, 16)
+# int8, scale (B, H, blocks, 2) float32, tail (B, H, 2, 2, 64, D) of the rows' type.
+KV8 = collections.namedtuple('KV8', 'k8 v8 scale tail')
+KV8_BLOCK = 64
+
+
+def kv8_cache(B, H, D, tokens, device, dtype=torch.bfloat16):
+    """An empty cache for B sequences of up to `tokens` tokens (rounded up to whole blocks), H KV heads of D = 64, 128 or 256."""
+    if D not in (64, 128, 256) or dtype not in (torch.bfloat16, torch.float16) or min(B, H, tokens) < 1:
+        raise ValueError('kv8_cache: at least one sequence, head and token, head size 64, 128 or 256, bfloat16 or float16 rows')
+    n = (tokens + KV8_BLOCK - 1) // KV8_BLOCK
+    i8 = dict(dtype=torch.int8, device=device)
+    return KV8(torch.zeros(B, H, n, 4, D // 16, 16, 16, **i8), torch.zeros(B, H, n, D // 16, 4, 16, 16, **i8),
+               torch.ones(B, H, n, 2, dtype=torch.float32, device=device), torch.zeros(B, H, 2, 2, KV8_BLOCK, D, dtype=dtype, device=device))
+
+
+def _kv8(cache, what):
+    """Sizes (B, H, D, blocks) of a cache whose tensors fit each other."""
+    k8, v8, scale, tail = cache
+    B, H, n = k8.shape[:3]
+    D = 16 * k8.shape[4]
+    if (tuple(k8.shape) != (B, H, n, 4, D // 16, 16, 16) or tuple(v8.shape) != (B, H, n, D // 16, 4, 16, 16) or tuple(scale.shape) != (B, H, n, 2)
+            or tuple(tail.shape) != (B, H, 2, 2, KV8_BLOCK, D) or k8.dtype != torch.int8 or v8.dtype != torch.int8 or scale.dtype != torch.float32):
+        raise ValueError(f'{what}: these tensors are not those of a kv8_cache')
+    _contig(k8, v8, scale, tail)
+    return B, H, D, n
+
+
+def _per_sequence(what, rows, B, cu, most, *counts):
+    """most of a call's sequences: rows / B without cu (equal counts), else given."""
+    for t in counts + (cu,):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1):
+            raise ValueError(f'{what}: counts and offsets are one-dimensional int32 tensors')
+    for t in counts:
+        if t.numel() != B:
+            raise ValueError(f'{what}: {t.numel()} counts for {B} sequences')
+    if cu is None:
+        if rows % B or most not in (None, rows // B):
+            raise ValueError(f'{what}: {rows} rows are not the same number for {B} sequences (give cu and most)')
+        return rows // B
+    if cu.numel() != B + 1 or most is None or most < 0:
+        raise ValueError(f'{what}: cu has one offset more than sequences, and most bounds their rows')
+    return min(most, rows)
+
+
+def kv8_append(cache, k, v, start, cu=None, most=None):
+    """Writes rows k, v (rows, H, D; the type of cache.tail, any token and head strides) into the cache from position start[b] (B, int32, on
+    the device) of every sequence on: B equal shares of the rows, or rows cu[b] .. cu[b + 1] - 1 (cu (B + 1,) int32 on the device, most: at
+    least the rows of any sequence). What was held from start[b] on is replaced; start[b] may lie up to 64 rows before the last
+    append's end. Rows past the capacity are dropped (see tcq_kv8_append)."""
+    B, H, D, n = _kv8(cache, 'kv8_append')
+    _heads(k, 'kv8_append k', D), _heads(v, 'kv8_append v', D)
+    rows = k.shape[0]
+    if k.shape != v.shape or k.shape[1] != H or k.dtype != cache.tail.dtype or v.dtype != k.dtype:
+        raise ValueError(f'kv8_append: k and v must be (rows, {H}, {D}) {cache.tail.dtype}')
+    most = _per_sequence('kv8_append', rows, B, cu, most, start)
+    _contig(start, cu)
+    _one_device('kv8_append', k, v, start, cu, *cache)
+    if rows == 0 or most == 0:
+        return
+    call('tcq_kv8_append', ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), _dt(k, (1, 2), 'kv8_append k'), ptr(cu), ptr(start),
+         rows, most, B, H, D, n, ptr(cache.k8), ptr(cache.v8), ptr(cache.scale), ptr(cache.tail), stream())
+
+
+def kv8_read(cache, first, lens, n, dtype=None):
+    """Rows first[b] .. first[b] + n - 1 of every sequence as the values that the cache stands for: k, v (B, n, H, D) of dtype (None: the
+    type of cache.tail), zeros from lens[b] on. first, lens (B,) int32 on the device."""
+    B, H, D, blocks = _kv8(cache, 'kv8_read')
+    _per_sequence('kv8_read', 0, B, None, None, first, lens)
+    _contig(first, lens)
+    _one_device('kv8_read', first, lens, *cache)
+    k, v = (torch.empty(B, n, H, D, dtype=dtype or cache.tail.dtype, device=cache.k8.device) for _ in range(2))
+    if n > 0:
+        call('tcq_kv8_read', ptr(cache.k8), ptr(cache.v8), ptr(cache.scale), ptr(first), ptr(lens), n, B, H, D, blocks, ptr(k), ptr(v),
+             _dt(k, (0, 1, 2), 'kv8_read'), stream())
+    return k, v
+
+
+def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=None, keys=None):
+    """Attention of q (rows, Hq, D; BF16 / FP16, any token and head strides) over the first lens[b] rows (int32, on the device) of every
+    sequence of the cache, Hq a multiple of its heads: o (rows, Hq, D). B equal shares of the rows, or cu and most as in kv8_append. With
+    causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended). scale: of the scores,
+    1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work alone."""
+    B, H, D, n = _kv8(cache, 'kv8_attend')
+    _heads(q, 'kv8_attend q', D)
+    rows, Hq = q.shape[:2]
+    if Hq == 0 or Hq % H:
+        raise ValueError(f'kv8_attend: {Hq} query heads over {H} key / value heads')
+    d = _dt(q, (1, 2), 'kv8_attend q')
+    most = _per_sequence('kv8_attend', rows, B, cu, most, lens)
+    if o is None:
+        o = torch.empty(rows, Hq, D, dtype=q.dtype, device=q.device)
+    elif o.shape != q.shape or o.dtype != q.dtype:
+        raise ValueError(f'kv8_attend: o must be {tuple(q.shape)} {q.dtype}')
+    _contig(o, lens, cu)
+    _one_device('kv8_attend', q, lens, cu, o, *cache)
+    if rows == 0 or most == 0:
+        return o
+    keys = n * KV8_BLOCK if keys is None else max(0, min(int(keys), n * KV8_BLOCK))
+    floats = _lib.lib().tcq_kv8_attend_floats(rows, most, B, Hq, H, D, keys)
+    part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    call('tcq_kv8_attend', ptr(q), q.stride(0), q.stride(1), d, ptr(cu), ptr(lens), rows, most, B, Hq, H, D, n, ptr(cache.k8), ptr(cache.v8),
+         ptr(cache.scale), int(causal), 1.0 / math.sqrt(D) if scale is None else float(scale), keys, ptr(part), ptr(o), stream())
+    return o
 
 
 # ------------------------------------------------------------------------------------------------------------- attention
