@@ -153,7 +153,8 @@ def ptr(t):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle: torch.cuda.current_stream().cuda_stream without the Stream object (2.9 -> 0.3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def call(name, *args):

@@ -287,11 +287,11 @@ def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offs
         raise ValueError(f'add_norm_quantize: q must be ({M}, {K}) int8')
     _q4_holds(q4, M, K, 'add_norm_quantize')
     _contig(w, q, q4, scale)
-    _one_device('add_norm_quantize', x, r, w, q, q4, scale, xout)
+    px, pr, pw, pq, p4, ps, po = _ptrs('add_norm_quantize', x, r, w, q, q4, scale, xout)
     if M == 0:
         return
-    call('tcq_add_norm_quantize', ptr(x), x.stride(0), ptr(r), 0 if r is None else r.stride(0), ptr(w), float(eps), float(offset), d,
-         ptr(xout), 0 if xout is None else xout.stride(0), ptr(q), ptr(q4), _ldq(q4), ptr(scale), M, K, stream())
+    call('tcq_add_norm_quantize', px, x.stride(0), pr, 0 if r is None else r.stride(0), pw, eps, offset, d, po,
+         0 if xout is None else xout.stride(0), pq, p4, _ldq(q4), ps, M, K, stream())
 
 
 def _q4_holds(q4, M, K, what):
@@ -306,16 +306,22 @@ def _q4_holds(q4, M, K, what):
         raise ValueError(f'{what}: q4 {tuple(q4.shape)} {q4.dtype} does not hold {M} tokens of {K} columns')
 
 
-def _one_device(what, *ts):
-    """The tensors of a call are on the current device: its stream is the one that the kernels run on."""
-    at = None
+def _ptrs(what, *ts):
+    """Device pointers of a call's tensors (None -> NULL), all on the current device: its stream is the one that the kernels run on."""
+    at, out = None, []
     for t in ts:
-        if t is not None:
-            if not t.is_cuda:
+        if t is None:
+            out.append(None)
+            continue
+        d = t.get_device()
+        if d != at:
+            if d < 0:
                 raise _lib.TcqError(f'{what}: libtcq takes device tensors only (got a CPU tensor)')
-            at = torch.cuda.current_device() if at is None else at
-            if t.get_device() != at:
-                raise ValueError(f'{what}: a tensor is on {t.device}, the current device is cuda:{at}')
+            at = torch.cuda.current_device()
+            if d != at:
+                raise ValueError(f'{what}: a tensor is on cuda:{d}, the current device is cuda:{at}')
+        out.append(t.data_ptr())
+    return out
 
 
 # --------------------------------------------------------------------------------------- rotary positions, the 8-bit cache
@@ -338,8 +344,10 @@ def rope_frequencies(R, theta=10000.0, sections=None, interleaved=False, device=
 
 
 def _heads(t, what, D=None):
-    if t.dim() != 3 or t.stride(2) != 1 or (D is not None and t.shape[2] != D):
-        raise ValueError(f'{what} must be (tokens, heads, {D or "D"}) with contiguous values, got {tuple(t.shape)}')
+    s = t.shape
+    if len(s) != 3 or t.stride(2) != 1 or (D is not None and s[2] != D):
+        raise ValueError(f'{what} must be (tokens, heads, {D or "D"}) with contiguous values, got {tuple(s)}')
+    return s
 
 
 def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False, inverse=False):
@@ -347,19 +355,20 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
     and head strides (views into a q | k | v row). pos (A, M) or (M,) int32 / int64; freq (R / 2,) float64 and axis (R / 2,) int32 as
     rope_frequencies makes them, the R first values of a head turn. Outputs None: in place. adjacent: pairs (2 i, 2 i + 1) instead of
     (i, i + R / 2). inverse: turns back, which is also the gradient."""
-    _heads(q, 'rope_axes q')
-    M, Hq, D = q.shape
-    q_out = q if q_out is None else q_out
+    M, Hq, D = _heads(q, 'rope_axes q')
+    qo = q if q_out is None else q_out
     d = _dt(q, (0, 1, 2), 'rope_axes q')
-    pairs = [(q, q_out)]
-    if k is not None:
-        k_out = k if k_out is None else k_out
-        _heads(k, 'rope_axes k', D)
-        pairs.append((k, k_out))
-    elif k_out is not None:
-        raise ValueError('rope_axes: k_out without k')
-    for x, y in pairs:
-        _heads(y, 'rope_axes outputs', D)
+    if k is None:
+        if k_out is not None:
+            raise ValueError('rope_axes: k_out without k')
+        ko, Hk = None, 0
+    else:
+        ko, Hk = k if k_out is None else k_out, _heads(k, 'rope_axes k', D)[1]
+    for x, y, H in ((q, qo, Hq), (k, ko, Hk)):
+        if x is None:
+            continue
+        if y is not x:
+            _heads(y, 'rope_axes outputs', D)
         if x.shape[0] != M or y.shape != x.shape or x.dtype != q.dtype or y.dtype != q.dtype:
             raise ValueError('rope_axes: q, k and their outputs must have the same tokens, head size and type')
     pos = pos[None] if pos.dim() == 1 else pos
@@ -369,13 +378,14 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
     if freq.dtype != torch.float64 or not 0 < R <= D or (axis is not None and (axis.dtype != torch.int32 or axis.numel() != R // 2)):
         raise ValueError(f'rope_axes: freq must be float64 of at most {D // 2} pairs and axis int32 of as many')
     _contig(freq, axis)
-    _one_device('rope_axes', q, k, pos, freq, axis, q_out, k_out)
+    pq, pk, pp, pf, pa, pqo, pko = _ptrs('rope_axes', q, k, pos, freq, axis, qo, ko)
     if M == 0:
-        return q_out, k_out
-    ks = (None, 0, 0, None, 0, 0, 0) if k is None else (ptr(k), k.stride(0), k.stride(1), ptr(k_out), k_out.stride(0), k_out.stride(1), k.shape[1])
-    call('tcq_rope_axes', ptr(q), q.stride(0), q.stride(1), ptr(q_out), q_out.stride(0), q_out.stride(1), Hq, *ks, d, ptr(pos),
-         int(pos.dtype == torch.int64), pos.stride(0), pos.stride(1), ptr(freq), ptr(axis), A, M, D, R, int(adjacent), int(inverse), stream())
-    return q_out, k_out
+        return qo, ko
+    sq, so, sp = q.stride(), qo.stride(), pos.stride()
+    sk, sko = ((0, 0), (0, 0)) if k is None else (k.stride(), ko.stride())
+    call('tcq_rope_axes', pq, sq[0], sq[1], pqo, so[0], so[1], Hq, pk, sk[0], sk[1], pko, sko[0], sko[1], Hk, d, pp, pos.dtype == torch.int64,
+         sp[0], sp[1], pf, pa, A, M, D, R, adjacent, inverse, stream())
+    return qo, ko
 
 
 # A cache of one attention layer in 8 bits (include/tcq_api.h): k8 (B, H, blocks, 4, D / 16, 16, 16) and v8 (B, H, blocks, D / 16, 4, 16, 16)
@@ -397,13 +407,14 @@ def kv8_cache(B, H, D, tokens, device, dtype=torch.bfloat16):
 def _kv8(cache, what):
     """Sizes (B, H, D, blocks) of a cache whose tensors fit each other."""
     k8, v8, scale, tail = cache
-    B, H, n = k8.shape[:3]
-    D = 16 * k8.shape[4]
-    if (tuple(k8.shape) != (B, H, n, 4, D // 16, 16, 16) or tuple(v8.shape) != (B, H, n, D // 16, 4, 16, 16) or tuple(scale.shape) != (B, H, n, 2)
-            or tuple(tail.shape) != (B, H, 2, 2, KV8_BLOCK, D) or k8.dtype != torch.int8 or v8.dtype != torch.int8 or scale.dtype != torch.float32):
+    if k8.dim() != 7:
+        raise ValueError(f'{what}: these tensors are not those of a kv8_cache')
+    B, H, n, _, E, _, _ = size = k8.shape
+    if (size != (B, H, n, 4, E, 16, 16) or v8.shape != (B, H, n, E, 4, 16, 16) or scale.shape != (B, H, n, 2)
+            or tail.shape != (B, H, 2, 2, KV8_BLOCK, 16 * E) or k8.dtype != torch.int8 or v8.dtype != torch.int8 or scale.dtype != torch.float32):
         raise ValueError(f'{what}: these tensors are not those of a kv8_cache')
     _contig(k8, v8, scale, tail)
-    return B, H, D, n
+    return B, H, 16 * E, n
 
 
 def _per_sequence(what, rows, B, cu, most, *counts):
@@ -429,17 +440,17 @@ def kv8_append(cache, k, v, start, cu=None, most=None):
     least the rows of any sequence). What was held from start[b] on is replaced; start[b] may lie up to 64 rows before the last
     append's end. Rows past the capacity are dropped (see tcq_kv8_append)."""
     B, H, D, n = _kv8(cache, 'kv8_append')
-    _heads(k, 'kv8_append k', D), _heads(v, 'kv8_append v', D)
-    rows = k.shape[0]
+    rows = _heads(k, 'kv8_append k', D)[0]
+    _heads(v, 'kv8_append v', D)
     if k.shape != v.shape or k.shape[1] != H or k.dtype != cache.tail.dtype or v.dtype != k.dtype:
         raise ValueError(f'kv8_append: k and v must be (rows, {H}, {D}) {cache.tail.dtype}')
     most = _per_sequence('kv8_append', rows, B, cu, most, start)
     _contig(start, cu)
-    _one_device('kv8_append', k, v, start, cu, *cache)
+    pk, pv, ps, pc, *pcache = _ptrs('kv8_append', k, v, start, cu, *cache)
     if rows == 0 or most == 0:
         return
-    call('tcq_kv8_append', ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), _dt(k, (1, 2), 'kv8_append k'), ptr(cu), ptr(start),
-         rows, most, B, H, D, n, ptr(cache.k8), ptr(cache.v8), ptr(cache.scale), ptr(cache.tail), stream())
+    sk, sv = k.stride(), v.stride()
+    call('tcq_kv8_append', pk, sk[0], sk[1], pv, sv[0], sv[1], _dt(k, (1, 2), 'kv8_append k'), pc, ps, rows, most, B, H, D, n, *pcache, stream())
 
 
 def kv8_read(cache, first, lens, n, dtype=None):
@@ -448,11 +459,10 @@ def kv8_read(cache, first, lens, n, dtype=None):
     B, H, D, blocks = _kv8(cache, 'kv8_read')
     _per_sequence('kv8_read', 0, B, None, None, first, lens)
     _contig(first, lens)
-    _one_device('kv8_read', first, lens, *cache)
+    pf, pl, pk8, pv8, ps, _ = _ptrs('kv8_read', first, lens, *cache)
     k, v = (torch.empty(B, n, H, D, dtype=dtype or cache.tail.dtype, device=cache.k8.device) for _ in range(2))
     if n > 0:
-        call('tcq_kv8_read', ptr(cache.k8), ptr(cache.v8), ptr(cache.scale), ptr(first), ptr(lens), n, B, H, D, blocks, ptr(k), ptr(v),
-             _dt(k, (0, 1, 2), 'kv8_read'), stream())
+        call('tcq_kv8_read', pk8, pv8, ps, pf, pl, n, B, H, D, blocks, k.data_ptr(), v.data_ptr(), _dt(k, (0, 1, 2), 'kv8_read'), stream())
     return k, v
 
 
@@ -462,8 +472,7 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
     causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended). scale: of the scores,
     1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work alone."""
     B, H, D, n = _kv8(cache, 'kv8_attend')
-    _heads(q, 'kv8_attend q', D)
-    rows, Hq = q.shape[:2]
+    rows, Hq, _ = _heads(q, 'kv8_attend q', D)
     if Hq == 0 or Hq % H:
         raise ValueError(f'kv8_attend: {Hq} query heads over {H} key / value heads')
     d = _dt(q, (1, 2), 'kv8_attend q')
@@ -473,14 +482,15 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
     elif o.shape != q.shape or o.dtype != q.dtype:
         raise ValueError(f'kv8_attend: o must be {tuple(q.shape)} {q.dtype}')
     _contig(o, lens, cu)
-    _one_device('kv8_attend', q, lens, cu, o, *cache)
+    pq, pl, pc, po, pk8, pv8, ps, _ = _ptrs('kv8_attend', q, lens, cu, o, *cache)
     if rows == 0 or most == 0:
         return o
     keys = n * KV8_BLOCK if keys is None else max(0, min(int(keys), n * KV8_BLOCK))
     floats = _lib.lib().tcq_kv8_attend_floats(rows, most, B, Hq, H, D, keys)
     part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    call('tcq_kv8_attend', ptr(q), q.stride(0), q.stride(1), d, ptr(cu), ptr(lens), rows, most, B, Hq, H, D, n, ptr(cache.k8), ptr(cache.v8),
-         ptr(cache.scale), int(causal), 1.0 / math.sqrt(D) if scale is None else float(scale), keys, ptr(part), ptr(o), stream())
+    sq = q.stride()
+    call('tcq_kv8_attend', pq, sq[0], sq[1], d, pc, pl, rows, most, B, Hq, H, D, n, pk8, pv8, ps, causal,
+         1.0 / math.sqrt(D) if scale is None else scale, keys, None if part is None else part.data_ptr(), po, stream())
     return o
 
 
