@@ -75,88 +75,80 @@ __device__ __forceinline__ void rope_table(const RopeArgs& a, int t0, int n, flo
     }
 }
 
-// grid ceil(M / TT): a workgroup's pieces are (token, head, piece of E pairs) with the piece index fastest, so a wave's loads
-// are runs of whole rows. ADJ: pairs are neighbours (2 i, 2 i + 1) and a piece is 16 bytes of E / 2 pairs; else they lie R / 2
-// apart and a piece is two times 16 bytes. The columns from R on are copied where the output is another tensor.
+// grid ceil(M / TT): the pieces (of E pairs) of a head on neighbouring threads, so a wave's loads are runs of whole rows; thread (g, c) takes
+// piece c of the head rows (token, head) g, g + G, ... of the workgroup's TT tokens, whose token and head it steps by the quotient and
+// remainder of G by the heads. ADJ: pairs are neighbours (2 i, 2 i + 1) and a piece is 16 bytes of E / 2 pairs; else they lie R / 2 apart
+// and a piece is two times 16 bytes. The columns from R on are copied where the output is another tensor.
 template <int DT, bool ADJ>
 __global__ __launch_bounds__(RT) void k_rope(RopeArgs a, int TT) {
-    constexpr int ES = DT == TCQ_F32 ? 4 : 2, E = 16 / ES;
+    constexpr int ES = DT == TCQ_F32 ? 4 : 2, E = 16 / ES, N = ADJ ? 1 : 2;
     __shared__ __attribute__((aligned(16))) float2_t cs[RTAB];
     const int half = a.R >> 1, t0 = blockIdx.x * TT, n = min(TT, a.M - t0), H = a.p[0].heads + a.p[1].heads;
-    const int NP = ADJ ? a.R / E : half / E, NR = (a.D - a.R) / E, per = H * NP, units = n * per;
-    auto where = [&](int u, int& t, int& f, const char*& x, char*& y) {
-        t = u / per;
-        const int w = u - t * per, h = w / NP, c = w - h * NP;
-        f = ADJ ? c * (E / 2) : c * E;
-        const bool second = h >= a.p[0].heads;
-        const RopeHeads& p = a.p[second];
-        const int hh = second ? h - a.p[0].heads : h;
-        const int64_t at = (int64_t)c * 16;
-        x = p.x + (t0 + t) * p.x_tok + hh * p.x_head + at;
-        y = p.y + (t0 + t) * p.y_tok + hh * p.y_head + at;
-    };
-    uint4_t v[RU][ADJ ? 1 : 2];
-    auto load = [&](int u0) {
+    const int NP = ADJ ? a.R / E : half / E, G = RT / NP, c = threadIdx.x % NP, g = threadIdx.x / NP, dt = G / H, dh = G - dt * H;
+    int t = g < G ? g / H : n, h = g - t * H;                             // (threads past the last whole group have no rows)
+    const float2_t* tab = cs + (ADJ ? c * (E / 2) : c * E);
+    uint4_t v[RU][N];
+    char* out[RU];
+    int tt[RU];
+    auto load = [&] {
 #pragma unroll
         for (int i = 0; i < RU; ++i) {
-            const int u = u0 + i * RT;
-            if (u >= units) break;
-            int t, f;
-            const char* x;
-            char* y;
-            where(u, t, f, x, y);
-            v[i][0] = *gptr((const uint4_t*)x);
-            if (!ADJ) v[i][ADJ ? 0 : 1] = *gptr((const uint4_t*)(x + (size_t)half * ES));
+            tt[i] = t;
+            if (t < n) {
+                const bool second = h >= a.p[0].heads;
+                const RopeHeads& p = a.p[second];
+                const int hh = second ? h - a.p[0].heads : h;
+                const char* x = p.x + (t0 + t) * p.x_tok + hh * p.x_head + c * 16;
+                out[i] = p.y + (t0 + t) * p.y_tok + hh * p.y_head + c * 16;
+#pragma unroll
+                for (int k = 0; k < N; ++k) v[i][k] = *gptr((const uint4_t*)(x + (size_t)(k * half * ES)));
+            }
+            t += dt;
+            h += dh;
+            if (h >= H) h -= H, ++t;
         }
     };
-    load(threadIdx.x);
+    load();
     rope_table(a, t0, n, cs);
     __syncthreads();
-    for (int u0 = threadIdx.x; u0 < units; u0 += RU * RT) {
-        if (u0 != (int)threadIdx.x) load(u0);
+    for (;;) {
 #pragma unroll
         for (int i = 0; i < RU; ++i) {
-            const int u = u0 + i * RT;
-            if (u >= units) break;
-            int t, f;
-            const char* x;
-            char* y;
-            where(u, t, f, x, y);
-            const float2_t* tab = cs + t * half + f;
+            if (tt[i] >= n) break;
+            const float2_t* w = tab + tt[i] * half;
             float p[E], q[E];
             rope_unpack<DT>(v[i][0], p);
             if constexpr (ADJ) {
 #pragma unroll
                 for (int k = 0; k < E; k += 2) {
-                    const float2_t w = tab[k >> 1];
                     const float lo = p[k], hi = p[k + 1];
-                    p[k] = __builtin_fmaf(lo, w.x, -(hi * w.y));
-                    p[k + 1] = __builtin_fmaf(hi, w.x, lo * w.y);
+                    p[k] = __builtin_fmaf(lo, w[k >> 1].x, -(hi * w[k >> 1].y));
+                    p[k + 1] = __builtin_fmaf(hi, w[k >> 1].x, lo * w[k >> 1].y);
                 }
-                *gptr((uint4_t*)y) = rope_pack<DT>(p);
             } else {
-                rope_unpack<DT>(v[i][ADJ ? 0 : 1], q);
+                rope_unpack<DT>(v[i][N - 1], q);
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
-                    const float2_t w = tab[k];
                     const float lo = p[k], hi = q[k];
-                    p[k] = __builtin_fmaf(lo, w.x, -(hi * w.y));
-                    q[k] = __builtin_fmaf(hi, w.x, lo * w.y);
+                    p[k] = __builtin_fmaf(lo, w[k].x, -(hi * w[k].y));
+                    q[k] = __builtin_fmaf(hi, w[k].x, lo * w[k].y);
                 }
-                *gptr((uint4_t*)y) = rope_pack<DT>(p);
-                *gptr((uint4_t*)(y + (size_t)half * ES)) = rope_pack<DT>(q);
+                *gptr((uint4_t*)(out[i] + (size_t)(half * ES))) = rope_pack<DT>(q);
             }
+            *gptr((uint4_t*)out[i]) = rope_pack<DT>(p);
         }
+        if (t >= n) break;
+        load();
     }
-    const int rest = n * H * NR;
+    const int NR = (a.D - a.R) / E, rest = n * H * NR;
     for (int u = threadIdx.x; u < rest; u += RT) {
-        const int t = u / (H * NR), w = u - t * H * NR, h = w / NR, c = w - h * NR;
-        const bool second = h >= a.p[0].heads;
+        const int ut = u / (H * NR), w = u - ut * H * NR, uh = w / NR;
+        const bool second = uh >= a.p[0].heads;
         const RopeHeads& p = a.p[second];
-        const int hh = second ? h - a.p[0].heads : h;
-        const int64_t at = (int64_t)a.R * ES + (int64_t)c * 16;
-        const char* x = p.x + (t0 + t) * p.x_tok + hh * p.x_head + at;
-        char* y = p.y + (t0 + t) * p.y_tok + hh * p.y_head + at;
+        const int hh = second ? uh - a.p[0].heads : uh;
+        const int64_t at = (int64_t)a.R * ES + (int64_t)(w - uh * NR) * 16;
+        const char* x = p.x + (t0 + ut) * p.x_tok + hh * p.x_head + at;
+        char* y = p.y + (t0 + ut) * p.y_tok + hh * p.y_head + at;
         if (x != y) *gptr((uint4_t*)y) = *gptr((const uint4_t*)x);
     }
 }
@@ -209,6 +201,7 @@ void rope_launch(const RopeArgs& a, bool adj, bool vec, hipStream_t st) {
         launch_k(k_rope_any<DT>, dim3(a.M), dim3(RT), 0, st, a, (int)adj);
         return;
     }
+    // tokens a workgroup: about 1024 workgroups (2048 tokens of 24 heads x 128 BF16: 512 7.7 us, 1024 7.6, 2048 8.3; 4761 of 32 x 64 FP32 14.7 / 13.9 / 13.5)
     const int TT = max(1, min(RTAB / max(1, a.R >> 1), (a.M + 1023) / 1024));
     if (adj) launch_k(k_rope<DT, true>, dim3((a.M + TT - 1) / TT), dim3(RT), 0, st, a, TT);
     else launch_k(k_rope<DT, false>, dim3((a.M + TT - 1) / TT), dim3(RT), 0, st, a, TT);
@@ -241,7 +234,7 @@ extern "C" int tcq_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void*
     a.D = D;
     a.R = R;
     a.inverse = inverse;
-    bool vec = R / 2 <= RTAB && (D - R) % E == 0 && (adjacent ? R % E == 0 : R % (2 * E) == 0);
+    bool vec = R / 2 <= RTAB && R / 2 / E <= RT && (D - R) % E == 0 && (adjacent ? R % E == 0 : R % (2 * E) == 0);
     for (int i = 0; i < (Hk ? 2 : 1); ++i) {
         const RopeHeads& p = a.p[i];
         vec = vec && !(((uintptr_t)p.x | (uintptr_t)p.y) % 16) && !((p.x_tok | p.x_head | p.y_tok | p.y_head) % 16);

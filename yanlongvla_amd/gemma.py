@@ -76,7 +76,10 @@ class GemmaAttention(nn.Module):
 
     def core(self, q, k, v, cache_k=None, cache_v=None, causal_offset=None):
         """Attention of the projected q / k / v (the cache rows, if any, before this call's own keys / values). Device
-        BF16 tensors go to the HIP attention kernel; host tensors (CPU twins in tests) to the same formula in PyTorch."""
+        BF16 tensors go to the HIP attention kernel; host tensors (CPU twins in tests) to the same formula in PyTorch. cache_k may
+        be a kernels.KV8Rows: the rows then go into that 8-bit cache (causal_offset: its length, or None for every row to see all)."""
+        if hasattr(cache_k, 'core'):
+            return cache_k.core(q, k, v, self.heads, causal_offset is not None)
         if self._device(q):
             from . import kernels
             o = torch.empty(q.shape[0], self.heads * self.head_dim, dtype=torch.bfloat16, device=q.device)
@@ -157,6 +160,50 @@ class KVCache:
             raise RuntimeError(f'KV cache full ({P} rows)')
         return self.k[i][:P], self.v[i][:P], (self.k[i][P:P + 1], self.v[i][P:P + 1])
 
+    def advance(self):
+        """Counts the row that a decode step has written in every layer."""
+        self.length += 1
+
+
+class KV8Cache:
+    """KVCache with its rows held in 8 bits (kernels.kv8_cache: half the memory, and half the bytes that a decode step reads), one scale
+    for every 64 rows. The length lives on the device as well, and a step's kernels take it from there: a captured decode step
+    can be replayed and goes on to the next position by itself (the host's count, which rows() checks against the capacity, does
+    not see replays: rows past the capacity are dropped). rewind() returns to the rows given at construction, which takes
+    their last block's rows from `ks` and `vs` again."""
+
+    def __init__(self, ks, vs, room):
+        from . import kernels
+        self.base = self.length = ks[0].shape[0]
+        self.cap = self.base + room
+        dev, D = ks[0].device, ks[0].shape[1]
+        self.start = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.caches = [kernels.kv8_cache(1, 1, D, self.cap, dev, k.dtype) for k in ks]
+        for c, k, v in zip(self.caches, ks, vs):
+            kernels.kv8_append(c, k.contiguous()[:, None], v.contiguous()[:, None], self.start)
+        tail = self.base // kernels.KV8_BLOCK * kernels.KV8_BLOCK
+        self.last = [(k[tail:].clone()[:, None], v[tail:].clone()[:, None]) for k, v in zip(ks, vs)]
+        self.start.fill_(self.base)
+
+    def rewind(self):
+        from . import kernels
+        tail = torch.full_like(self.start, self.base - self.last[0][0].shape[0])
+        for c, (k, v) in zip(self.caches, self.last):
+            kernels.kv8_append(c, k, v, tail)
+        self.start.fill_(self.base)
+        self.length = self.base
+
+    def rows(self, i):
+        """Layer i's cache as the layers take it: (kernels.KV8Rows, None, None)."""
+        from . import kernels
+        if self.length >= self.cap:
+            raise RuntimeError(f'KV cache full ({self.length} rows)')
+        return kernels.KV8Rows(self.caches[i], self.start), None, None
+
+    def advance(self):
+        self.length += 1
+        self.start.add_(1)
+
 
 EXPERT = dict(layers=18, width=1024, hidden=4096, heads=8, head_dim=256, action_dim=32)
 BACKBONE = dict(layers=18, width=2048, hidden=16384, heads=8, head_dim=256, vocab=257152)
@@ -179,7 +226,8 @@ class ExpertPolicy(nn.Module):
         return self.paligemma_with_expert.gemma_expert.model
 
     def set_prefix(self, ks, vs):
-        """Per-layer prefix keys / values (T, head_dim), as the backbone's prefill leaves them."""
+        """Per-layer prefix keys / values (T, head_dim), as the backbone's prefill leaves them; or, with vs all None, a kernels.KV8Rows
+        per layer whose start is the prefix's length (the action tokens of a step, at most 64, replace those of the step before)."""
         self.prefix_k, self.prefix_v = list(ks), list(vs)
 
     def velocity(self, x_t):
@@ -226,14 +274,15 @@ class BackbonePolicy(nn.Module):
         return self.stack.norm(h), ks, vs
 
     def decode_step_cached(self, x, cache):
-        """decode_step on a KVCache: the same hidden state, with this token's keys / values written into the cache."""
+        """decode_step on a KVCache: the same hidden state, with this token's keys / values written into the cache. On a KV8Cache: over
+        the rows that its 8 bits stand for."""
         from . import modules
         h = x
         with modules.deferred_outputs():                 # each layer's output goes straight to the next layer
             for i, layer in enumerate(self.stack.layers):
                 ck, cv, out = cache.rows(i)
                 h, _, _ = layer(h, ck, cv, kv_out=out)
-        cache.length += 1
+        cache.advance()
         return self.stack.norm(h)
 
     def decode_step(self, x, ks, vs):

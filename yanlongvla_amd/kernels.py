@@ -494,6 +494,23 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
     return o
 
 
+class KV8Rows:
+    """An 8-bit cache as a decoder layer takes it in the place of its key rows (gemma.KV8Cache.rows): the layer's KV8 of one sequence, the
+    position that this call's rows go to (start, (1,) int32 on the device) and, when `lens` is given, the length after them (else it is
+    made per call). core() appends the rows and attends over the whole: a later call with the same start replaces them, as long as they
+    are at most 64 (the action tokens of a denoising step)."""
+
+    def __init__(self, cache, start, lens=None, keys=None):
+        self.cache, self.start, self.lens, self.keys = cache, start, lens, keys
+
+    def core(self, q, k, v, heads, causal):
+        """Attention of q (M, heads * D) after k, v (M, H * D): o (M, heads * D)."""
+        M, D = q.shape[0], 16 * self.cache.k8.shape[4]
+        kv8_append(self.cache, k.reshape(M, -1, D), v.reshape(M, -1, D), self.start)
+        lens = self.start + M if self.lens is None else self.lens
+        return kv8_attend(q.reshape(M, heads, D), self.cache, lens, causal=causal, keys=self.keys).view(M, heads * D)
+
+
 # ------------------------------------------------------------------------------------------------------------- attention
 def attend(q, k_cache, v_cache, k_new, v_new, heads, causal_offset=None, o=None, su=None, q8=None, scale=None, q4=None):
     """Multi-query attention (H <= 8 heads, head dim 256), BF16: keys / values = cache rows (or None) then the new rows.

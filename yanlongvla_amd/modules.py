@@ -666,7 +666,8 @@ class KDecoderLayer(torch.nn.Module):
             else:
                 STATS['chained_prologues'] += 1
             z1 = qkv.product(b)
-        if self._attn_post_fits(M, z1, qkv, og, cache_k, cache_v):
+        in8 = isinstance(cache_k, kernels.KV8Rows)        # an 8-bit cache: its own append and attention, then the o projection's prologue
+        if not in8 and self._attn_post_fits(M, z1, qkv, og, cache_k, cache_v):
             # one token: the q/k/v epilogue runs inside the attention's launch (the query row never leaves it; the new key /
             # value rows go to kv_out), the chunk merge + o rotate + quantize inside the o product's launch
             a = self.self_attn
@@ -681,14 +682,14 @@ class KDecoderLayer(torch.nn.Module):
             STATS['attn_prologues'] += 1
         else:
             q, k, v = qkv.posts(z1, b, x2.shape, outs=None if kv_out is None else [None, kv_out[0], kv_out[1]])
-            if self._attn_prologue_fits(M, q, og):
+            if not in8 and self._attn_prologue_fits(M, q, og):
                 # one token: the attention's chunk merge + o rotate + quantize run inside the o product's launch
                 parts = self.self_attn.core_parts(q, k, v, cache_k, cache_v, causal_offset)
                 b2 = dict(q=None, q4=None, scale=torch.empty(M, dtype=torch.float32, device=dev))
                 z = og.product(None, og.k_parts(M), pro=kernels.prologue_attn(parts, self.self_attn.heads, og.su, scale=b2['scale']))
                 STATS['attn_prologues'] += 1
             else:
-                if hasattr(self.self_attn, 'core_quantized') and self.self_attn._device(q):
+                if not in8 and hasattr(self.self_attn, 'core_quantized') and self.self_attn._device(q):
                     b2 = og.buffers(M, dev)
                     self.self_attn.core_quantized(q, k, v, cache_k, cache_v, causal_offset, og.su, b2['q'], b2['scale'],
                                                   q4=b2['q4'])
