@@ -157,11 +157,14 @@ def stream():
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def failed(name, rc):
+    raise TcqError(f'{name} failed: {STATUS.get(rc, f"HIP error {rc}")} (status {rc})')
+
+
 def call(name, *args):
     rc = getattr(lib(), name)(*args)
     if rc != 0:
-        what = STATUS.get(rc, f'HIP error {rc}')
-        raise TcqError(f'{name} failed: {what} (status {rc})')
+        failed(name, rc)
     return rc
 
 

@@ -4,7 +4,6 @@ functions added here (rht, pre_h16, quantize_rows, repack, decode_f16, gemv_f16,
 """
 import collections
 import ctypes
-import math
 
 import torch
 
@@ -272,26 +271,26 @@ def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offs
     """h = x + r (r None: x), rounded to x's type and stored in xout where that is given (it may be x or r), then INT8 rows of
     RMSNorm(h) * (offset + w): q (M, K) int8 and / or q4 (as in pre), scale (M,) FP32, what gemm_i8 takes. x, r, xout (M, K) BF16 / FP16
     / FP32 with contiguous rows of any stride, w (K,) of that type; offset 1: Gemma's weights, 0: plain ones."""
-    M, K = x.shape
-    d = _dt(x, (0, 1, 2), 'add_norm_quantize x')
-    for t in (r, xout):
-        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.stride(1) != 1 and K > 1):
-            raise ValueError(f'add_norm_quantize: r and xout must be ({M}, {K}) {x.dtype} with contiguous rows')
-    if w.dtype != x.dtype or w.numel() != K or (x.stride(1) != 1 and K > 1):
-        raise ValueError(f'add_norm_quantize: w must be ({K},) {x.dtype}, the rows of x contiguous')
-    if scale is None or scale.dtype != torch.float32 or scale.numel() != M:
-        raise ValueError(f'add_norm_quantize: scale must be ({M},) float32')
-    if q is None and q4 is None:
-        raise ValueError('add_norm_quantize: q and / or q4')
-    if q is not None and (q.dtype != torch.int8 or q.shape != x.shape):
-        raise ValueError(f'add_norm_quantize: q must be ({M}, {K}) int8')
+    size, dt = x.shape, x.dtype
+    M, K = size
+    if dt not in DTYPE or dt not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f'add_norm_quantize x: unsupported dtype {dt}')
+    for t in (x, r, xout):
+        if t is not None and not (t.shape == size and t.dtype == dt and (t.stride(1) == 1 or K == 1)):
+            raise ValueError(f'add_norm_quantize: x, r and xout must be ({M}, {K}) {dt} with contiguous rows')
+    if w.dtype != dt or w.numel() != K or not w.is_contiguous():
+        raise ValueError(f'add_norm_quantize: w must be ({K},) {dt}, contiguous')
+    if scale is None or scale.dtype != torch.float32 or scale.numel() != M or not scale.is_contiguous():
+        raise ValueError(f'add_norm_quantize: scale must be ({M},) float32, contiguous')
+    if (q is None and q4 is None) or (q is not None and not (q.dtype == torch.int8 and q.shape == size and q.is_contiguous())):
+        raise ValueError(f'add_norm_quantize: q must be ({M}, {K}) int8, contiguous, or q4 given')
     _q4_holds(q4, M, K, 'add_norm_quantize')
-    _contig(w, q, q4, scale)
     px, pr, pw, pq, p4, ps, po = _ptrs('add_norm_quantize', x, r, w, q, q4, scale, xout)
-    if M == 0:
-        return
-    call('tcq_add_norm_quantize', px, x.stride(0), pr, 0 if r is None else r.stride(0), pw, eps, offset, d, po,
-         0 if xout is None else xout.stride(0), pq, p4, _ldq(q4), ps, M, K, stream())
+    if M:
+        rc = _lib.lib().tcq_add_norm_quantize(px, x.stride(0), pr, 0 if r is None else r.stride(0), pw, eps, offset, DTYPE[dt], po,
+                                              0 if xout is None else xout.stride(0), pq, p4, _ldq(q4), ps, M, K, stream())
+        if rc:
+            _lib.failed('tcq_add_norm_quantize', rc)
 
 
 def _q4_holds(q4, M, K, what):
@@ -302,24 +301,22 @@ def _q4_holds(q4, M, K, what):
         ok = q4.dtype == torch.int8 and tuple(q4.shape) == ((M + 15) // 16, K // 16, 16, 16) and K % 16 == 0
     else:
         ok = q4.dtype == torch.int32 and q4.dim() == 2 and 4 * q4.shape[0] == K and q4.shape[1] >= M
-    if not ok:
+    if not ok or not q4.is_contiguous():
         raise ValueError(f'{what}: q4 {tuple(q4.shape)} {q4.dtype} does not hold {M} tokens of {K} columns')
 
 
 def _ptrs(what, *ts):
     """Device pointers of a call's tensors (None -> NULL), all on the current device: its stream is the one that the kernels run on."""
-    at, out = None, []
+    at, out = torch.cuda.current_device() if ts[0].is_cuda else -1, []
     for t in ts:
         if t is None:
             out.append(None)
             continue
         d = t.get_device()
-        if d != at:
+        if d != at or d < 0:
             if d < 0:
                 raise _lib.TcqError(f'{what}: libtcq takes device tensors only (got a CPU tensor)')
-            at = torch.cuda.current_device()
-            if d != at:
-                raise ValueError(f'{what}: a tensor is on cuda:{d}, the current device is cuda:{at}')
+            raise ValueError(f'{what}: a tensor is on cuda:{d}, the current device is cuda:{torch.cuda.current_device()}')
         out.append(t.data_ptr())
     return out
 
@@ -355,37 +352,54 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
     and head strides (views into a q | k | v row). pos (A, M) or (M,) int32 / int64; freq (R / 2,) float64 and axis (R / 2,) int32 as
     rope_frequencies makes them, the R first values of a head turn. Outputs None: in place. adjacent: pairs (2 i, 2 i + 1) instead of
     (i, i + R / 2). inverse: turns back, which is also the gradient."""
-    M, Hq, D = _heads(q, 'rope_axes q')
-    qo = q if q_out is None else q_out
-    d = _dt(q, (0, 1, 2), 'rope_axes q')
+    if q_out is None:
+        q_out = q
     if k is None:
+        ko = None
+    else:
+        ko = k if k_out is None else k_out
+    size, ps, dt = q.shape, pos.shape, q.dtype
+    sq, so, sp = q.stride(), q_out.stride(), pos.stride()
+    if len(ps) == 1:
+        ps, sp = (1, *ps), (0, *sp)
+    half, wide = freq.numel(), pos.dtype
+    if not (len(size) == 3 and size == q_out.shape and q_out.dtype == dt in _ROPE_TYPES and sq[2] == so[2] == 1 and len(ps) == 2
+            and ps[1] == size[0] and (wide == torch.int32 or wide == torch.int64) and freq.dtype == torch.float64 and 0 < 2 * half <= size[2]
+            and freq.is_contiguous()
+            and (axis is None or (axis.dtype == torch.int32 and axis.numel() == half and axis.is_contiguous()))):
+        _rope_refuse(q, q_out, pos, freq, axis)
+    M, Hq, D = size
+    if ko is None:
         if k_out is not None:
             raise ValueError('rope_axes: k_out without k')
-        ko, Hk = None, 0
+        Hk, sk, sko = 0, (0, 0), (0, 0)
     else:
-        ko, Hk = k if k_out is None else k_out, _heads(k, 'rope_axes k', D)[1]
-    for x, y, H in ((q, qo, Hq), (k, ko, Hk)):
-        if x is None:
-            continue
-        if y is not x:
-            _heads(y, 'rope_axes outputs', D)
-        if x.shape[0] != M or y.shape != x.shape or x.dtype != q.dtype or y.dtype != q.dtype:
-            raise ValueError('rope_axes: q, k and their outputs must have the same tokens, head size and type')
-    pos = pos[None] if pos.dim() == 1 else pos
-    A, R = pos.shape[0], 2 * freq.numel()
-    if pos.dim() != 2 or pos.shape[1] != M or pos.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f'rope_axes: pos must be (axes, {M}) int32 or int64, got {tuple(pos.shape)} {pos.dtype}')
-    if freq.dtype != torch.float64 or not 0 < R <= D or (axis is not None and (axis.dtype != torch.int32 or axis.numel() != R // 2)):
-        raise ValueError(f'rope_axes: freq must be float64 of at most {D // 2} pairs and axis int32 of as many')
-    _contig(freq, axis)
-    pq, pk, pp, pf, pa, pqo, pko = _ptrs('rope_axes', q, k, pos, freq, axis, qo, ko)
-    if M == 0:
-        return qo, ko
-    sq, so, sp = q.stride(), qo.stride(), pos.stride()
-    sk, sko = ((0, 0), (0, 0)) if k is None else (k.stride(), ko.stride())
-    call('tcq_rope_axes', pq, sq[0], sq[1], pqo, so[0], so[1], Hq, pk, sk[0], sk[1], pko, sko[0], sko[1], Hk, d, pp, pos.dtype == torch.int64,
-         sp[0], sp[1], pf, pa, A, M, D, R, adjacent, inverse, stream())
-    return qo, ko
+        ks, sk, sko = k.shape, k.stride(), ko.stride()
+        if not (len(ks) == 3 and ks == ko.shape and ks[0] == M and ks[2] == D and k.dtype == ko.dtype == dt and sk[2] == sko[2] == 1):
+            raise ValueError(f'rope_axes: k and its output must be ({M}, heads, {D}) {dt} with contiguous values')
+        Hk = ks[1]
+    pq, pk, pp, pf, pa, pqo, pko = _ptrs('rope_axes', q, k, pos, freq, axis, q_out, ko)
+    if M:
+        rc = _lib.lib().tcq_rope_axes(pq, sq[0], sq[1], pqo, so[0], so[1], Hq, pk, sk[0], sk[1], pko, sko[0], sko[1], Hk, DTYPE[dt], pp,
+                                      wide == torch.int64, sp[0], sp[1], pf, pa, ps[0], M, D, 2 * half, adjacent, inverse, stream())
+        if rc:
+            _lib.failed('tcq_rope_axes', rc)
+    return q_out, ko
+
+
+_ROPE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _rope_refuse(q, q_out, pos, freq, axis):
+    """What rope_axes does not take of these."""
+    _heads(q, 'rope_axes q')
+    _dt(q, (0, 1, 2), 'rope_axes q')
+    _heads(q_out, 'rope_axes q_out', q.shape[2])
+    if q_out.shape != q.shape or q_out.dtype != q.dtype:
+        raise ValueError('rope_axes: q and its output must have the same size and type')
+    if pos.dim() not in (1, 2) or pos.shape[-1] != q.shape[0] or pos.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f'rope_axes: pos must be (axes, {q.shape[0]}) int32 or int64, got {tuple(pos.shape)} {pos.dtype}')
+    raise ValueError(f'rope_axes: freq must be contiguous float64 of at most {q.shape[2] // 2} pairs and axis int32 of as many')
 
 
 # A cache of one attention layer in 8 bits (include/tcq_api.h): k8 (B, H, blocks, 4, D / 16, 16, 16) and v8 (B, H, blocks, D / 16, 4, 16, 16)
@@ -405,33 +419,34 @@ def kv8_cache(B, H, D, tokens, device, dtype=torch.bfloat16):
 
 
 def _kv8(cache, what):
-    """Sizes (B, H, D, blocks) of a cache whose tensors fit each other."""
+    """Sizes (B, H, blocks, D / 16) of a cache whose tensors fit each other."""
     k8, v8, scale, tail = cache
-    if k8.dim() != 7:
-        raise ValueError(f'{what}: these tensors are not those of a kv8_cache')
-    B, H, n, _, E, _, _ = size = k8.shape
-    if (size != (B, H, n, 4, E, 16, 16) or v8.shape != (B, H, n, E, 4, 16, 16) or scale.shape != (B, H, n, 2)
-            or tail.shape != (B, H, 2, 2, KV8_BLOCK, 16 * E) or k8.dtype != torch.int8 or v8.dtype != torch.int8 or scale.dtype != torch.float32):
-        raise ValueError(f'{what}: these tensors are not those of a kv8_cache')
-    _contig(k8, v8, scale, tail)
-    return B, H, 16 * E, n
+    size = k8.shape
+    if len(size) == 7:
+        B, H, n, _, E, _, _ = size
+        if (size == (B, H, n, 4, E, 16, 16) and v8.shape == (B, H, n, E, 4, 16, 16) and scale.shape == (B, H, n, 2)
+                and tail.shape == (B, H, 2, 2, KV8_BLOCK, 16 * E) and k8.dtype == v8.dtype == torch.int8 and scale.dtype == torch.float32
+                and k8.is_contiguous() and v8.is_contiguous() and scale.is_contiguous() and tail.is_contiguous()):
+            return B, H, n, E
+    raise ValueError(f'{what}: these tensors are not those of a kv8_cache')
 
 
-def _per_sequence(what, rows, B, cu, most, *counts):
-    """most of a call's sequences: rows / B without cu (equal counts), else given."""
-    for t in counts + (cu,):
-        if t is not None and (t.dtype != torch.int32 or t.dim() != 1):
-            raise ValueError(f'{what}: counts and offsets are one-dimensional int32 tensors')
-    for t in counts:
-        if t.numel() != B:
-            raise ValueError(f'{what}: {t.numel()} counts for {B} sequences')
+def _counts(what, t, n):
+    """t: a contiguous one-dimensional int32 tensor of n values."""
+    if not (t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous()):
+        raise ValueError(f'{what}: counts and offsets are contiguous int32 tensors, one value for each sequence (cu: one more)')
+
+
+def _most(what, rows, B, cu, most):
+    """The most rows of a call's sequences: rows / B without cu (equal counts), else given."""
     if cu is None:
         if rows % B or most not in (None, rows // B):
             raise ValueError(f'{what}: {rows} rows are not the same number for {B} sequences (give cu and most)')
         return rows // B
-    if cu.numel() != B + 1 or most is None or most < 0:
-        raise ValueError(f'{what}: cu has one offset more than sequences, and most bounds their rows')
-    return min(most, rows)
+    _counts(what, cu, B + 1)
+    if most is None or most < 0:
+        raise ValueError(f'{what}: most bounds the rows of the sequences that cu gives')
+    return most if most < rows else rows
 
 
 def kv8_append(cache, k, v, start, cu=None, most=None):
@@ -439,30 +454,38 @@ def kv8_append(cache, k, v, start, cu=None, most=None):
     the device) of every sequence on: B equal shares of the rows, or rows cu[b] .. cu[b + 1] - 1 (cu (B + 1,) int32 on the device, most: at
     least the rows of any sequence). What was held from start[b] on is replaced; start[b] may lie up to 64 rows before the last
     append's end. Rows past the capacity are dropped (see tcq_kv8_append)."""
-    B, H, D, n = _kv8(cache, 'kv8_append')
-    rows = _heads(k, 'kv8_append k', D)[0]
-    _heads(v, 'kv8_append v', D)
-    if k.shape != v.shape or k.shape[1] != H or k.dtype != cache.tail.dtype or v.dtype != k.dtype:
-        raise ValueError(f'kv8_append: k and v must be (rows, {H}, {D}) {cache.tail.dtype}')
-    most = _per_sequence('kv8_append', rows, B, cu, most, start)
-    _contig(start, cu)
-    pk, pv, ps, pc, *pcache = _ptrs('kv8_append', k, v, start, cu, *cache)
-    if rows == 0 or most == 0:
-        return
-    sk, sv = k.stride(), v.stride()
-    call('tcq_kv8_append', pk, sk[0], sk[1], pv, sv[0], sv[1], _dt(k, (1, 2), 'kv8_append k'), pc, ps, rows, most, B, H, D, n, *pcache, stream())
+    B, H, n, E = _kv8(cache, 'kv8_append')
+    size, sk, sv, dt = k.shape, k.stride(), v.stride(), k.dtype
+    if not (len(size) == 3 and size == v.shape and size[1] == H and size[2] == 16 * E and sk[2] == sv[2] == 1 and dt == v.dtype == cache.tail.dtype
+            and dt in (torch.bfloat16, torch.float16)):
+        raise ValueError(f'kv8_append: k and v must be (rows, {H}, {16 * E}) {cache.tail.dtype} with contiguous values')
+    rows = size[0]
+    _counts('kv8_append', start, B)
+    most = _most('kv8_append', rows, B, cu, most)
+    pk, pv, ps, pc, pk8, pv8, pscale, ptail = _ptrs('kv8_append', k, v, start, cu, *cache)
+    if most and rows:
+        rc = _lib.lib().tcq_kv8_append(pk, sk[0], sk[1], pv, sv[0], sv[1], DTYPE[dt], pc, ps, rows, most, B, H, 16 * E, n, pk8, pv8, pscale, ptail,
+                                       stream())
+        if rc:
+            _lib.failed('tcq_kv8_append', rc)
 
 
 def kv8_read(cache, first, lens, n, dtype=None):
     """Rows first[b] .. first[b] + n - 1 of every sequence as the values that the cache stands for: k, v (B, n, H, D) of dtype (None: the
     type of cache.tail), zeros from lens[b] on. first, lens (B,) int32 on the device."""
-    B, H, D, blocks = _kv8(cache, 'kv8_read')
-    _per_sequence('kv8_read', 0, B, None, None, first, lens)
-    _contig(first, lens)
-    pf, pl, pk8, pv8, ps, _ = _ptrs('kv8_read', first, lens, *cache)
-    k, v = (torch.empty(B, n, H, D, dtype=dtype or cache.tail.dtype, device=cache.k8.device) for _ in range(2))
+    B, H, blocks, E = _kv8(cache, 'kv8_read')
+    _counts('kv8_read', first, B)
+    _counts('kv8_read', lens, B)
+    pf, pl, pk8, pv8, ps = _ptrs('kv8_read', first, lens, cache.k8, cache.v8, cache.scale)
+    dt = dtype or cache.tail.dtype
+    if dt not in _ROPE_TYPES:
+        raise TypeError(f'kv8_read: unsupported dtype {dt}')
+    size, dev = (B, n, H, 16 * E), cache.k8.device
+    k, v = torch.empty(size, dtype=dt, device=dev), torch.empty(size, dtype=dt, device=dev)
     if n > 0:
-        call('tcq_kv8_read', pk8, pv8, ps, pf, pl, n, B, H, D, blocks, k.data_ptr(), v.data_ptr(), _dt(k, (0, 1, 2), 'kv8_read'), stream())
+        rc = _lib.lib().tcq_kv8_read(pk8, pv8, ps, pf, pl, n, B, H, 16 * E, blocks, k.data_ptr(), v.data_ptr(), DTYPE[dt], stream())
+        if rc:
+            _lib.failed('tcq_kv8_read', rc)
     return k, v
 
 
@@ -471,26 +494,29 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
     sequence of the cache, Hq a multiple of its heads: o (rows, Hq, D). B equal shares of the rows, or cu and most as in kv8_append. With
     causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended). scale: of the scores,
     1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work alone."""
-    B, H, D, n = _kv8(cache, 'kv8_attend')
-    rows, Hq, _ = _heads(q, 'kv8_attend q', D)
-    if Hq == 0 or Hq % H:
-        raise ValueError(f'kv8_attend: {Hq} query heads over {H} key / value heads')
-    d = _dt(q, (1, 2), 'kv8_attend q')
-    most = _per_sequence('kv8_attend', rows, B, cu, most, lens)
+    B, H, n, E = _kv8(cache, 'kv8_attend')
+    size, sq, dt = q.shape, q.stride(), q.dtype
+    if not (len(size) == 3 and size[2] == 16 * E and sq[2] == 1 and size[1] > 0 and size[1] % H == 0):
+        raise ValueError(f'kv8_attend: q must be (rows, a multiple of {H} heads, {16 * E}) with contiguous values, got {tuple(size)}')
+    if dt != torch.bfloat16 and dt != torch.float16:
+        raise TypeError(f'kv8_attend q: unsupported dtype {dt}')
+    rows, Hq, D = size
+    _counts('kv8_attend', lens, B)
+    most = _most('kv8_attend', rows, B, cu, most)
     if o is None:
-        o = torch.empty(rows, Hq, D, dtype=q.dtype, device=q.device)
-    elif o.shape != q.shape or o.dtype != q.dtype:
-        raise ValueError(f'kv8_attend: o must be {tuple(q.shape)} {q.dtype}')
-    _contig(o, lens, cu)
-    pq, pl, pc, po, pk8, pv8, ps, _ = _ptrs('kv8_attend', q, lens, cu, o, *cache)
-    if rows == 0 or most == 0:
-        return o
-    keys = n * KV8_BLOCK if keys is None else max(0, min(int(keys), n * KV8_BLOCK))
-    floats = _lib.lib().tcq_kv8_attend_floats(rows, most, B, Hq, H, D, keys)
-    part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    sq = q.stride()
-    call('tcq_kv8_attend', pq, sq[0], sq[1], d, pc, pl, rows, most, B, Hq, H, D, n, pk8, pv8, ps, causal,
-         1.0 / math.sqrt(D) if scale is None else scale, keys, None if part is None else part.data_ptr(), po, stream())
+        o = torch.empty(size, dtype=dt, device=q.device)
+    elif o.shape != size or o.dtype != dt or not o.is_contiguous():
+        raise ValueError(f'kv8_attend: o must be contiguous {tuple(size)} {dt}')
+    pq, pl, pc, po, pk8, pv8, ps = _ptrs('kv8_attend', q, lens, cu, o, cache.k8, cache.v8, cache.scale)
+    if most and rows:
+        keys = n * KV8_BLOCK if keys is None else max(0, min(int(keys), n * KV8_BLOCK))
+        L = _lib.lib()
+        floats = L.tcq_kv8_attend_floats(rows, most, B, Hq, H, D, keys)
+        part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        rc = L.tcq_kv8_attend(pq, sq[0], sq[1], DTYPE[dt], pc, pl, rows, most, B, Hq, H, D, n, pk8, pv8, ps, causal,
+                              D ** -0.5 if scale is None else scale, keys, part.data_ptr() if floats else None, po, stream())
+        if rc:
+            _lib.failed('tcq_kv8_attend', rc)
     return o
 
 
