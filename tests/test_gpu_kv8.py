@@ -173,8 +173,10 @@ def reference(q, k, v, lens, counts, G, causal, scale=None):
     return out
 
 
-def close(o, want):
-    tol = torch.finfo(o.dtype).eps / 2 + 2e-4
+def close(o, want, score=0.0):
+    """score: the root mean square error of a score, for queries outside of what the 2e-4 covers: the probabilities' relative errors, and with
+    values of mean zero the outputs' (sum p^2 |v|^2 enters both norms)."""
+    tol = torch.finfo(o.dtype).eps / 2 + 2e-4 + score
     assert torch.isfinite(o).all()
     assert (o.double() - want).norm() <= tol * want.norm()
     assert (o.double() - want).abs().max() <= 8 * tol * want.abs().max()
@@ -196,6 +198,49 @@ def test_attend_matches_fp64(Hq, Hk, D, dt, lens, counts, causal):
     if len(set(counts)) == 1:
         p = K.kv8_attend(q, cache, ints(lens), causal=causal)
         assert torch.equal(o, p)
+
+
+@pytest.mark.parametrize('dt', [BF, HF])
+@pytest.mark.parametrize('lens,counts,causal', [([700, 420, 300, 64], [530, 420, 300, 1], True), ([333, 64], [1030, 1030], False)])
+def test_attend_of_many_rows(lens, counts, causal, dt):
+    """Enough rows for two tiles a wave: ragged ones, sequences shorter than their rows, rows that see nothing; blocks whose value scales
+    differ by up to 2^40, the largest where nothing looks."""
+    from yanlongvla_amd import kernels as K
+    Hq, Hk, D = 16, 8, 128
+    cache, _, _ = fill(lens, Hk, D, dt, seed=31)
+    q = rand(sum(counts), Hq, D, seed=32, dt=dt) * 2
+    q[5, 3, 7] = float('nan')
+    cu = ints([sum(counts[:i]) for i in range(len(counts) + 1)])
+    k, v = K.kv8_read(cache, ints([0] * len(lens)), ints(lens), max(lens), FP)
+    G = Hq // Hk
+
+    def both(cache, k, v, q):
+        o = torch.full_like(q, 9.0)
+        K.kv8_attend(q, cache, ints(lens), o, causal=causal, cu=cu, most=max(counts))
+        assert o[5, 3].isnan().all()
+        want = reference(q, k, v, lens, counts, G, causal)
+        o[5, 3], want[5, 3] = 0, 0
+        return o, want
+
+    close(*both(cache, k, v, q))
+    # the second block's values 2^-40 of the others', then 2^30 of them but with keys that no query picks
+    for e, pick in ((-40.0, False), (30.0, True)):
+        scale, k2, v2 = cache.scale.clone(), k.clone(), v.clone()
+        scale[:, :, 1, 1] *= 2.0 ** e
+        v2[:, T:2 * T] *= 2.0 ** e
+        qq = q.clone()
+        if pick:                                                        # one dim decides: no query picks the keys of that block
+            k8 = cache.k8.clone()
+            k8[:, :, :, :, 0, :, 0] = 127
+            k8[:, :, 1, :, 0, :, 0] = -127
+            big = K.KV8(k8, cache.v8, scale, cache.tail)
+            qq[..., 0] = 200.0
+            k2, _ = K.kv8_read(big, ints([0] * len(lens)), ints(lens), max(lens), FP)
+        else:
+            big = cache._replace(scale=scale)
+        # a digit of a query row whose largest value is 200 (2^E = 256) is off by at most half of 256 / 32512, 256 / 32512 / sqrt(12) =
+        # 2.3e-3 root mean square; keys of 128 normal values, one of them 127 codes of 4 / 127: norm 12; scale 1 / sqrt(128): 2.4e-3
+        close(*both(big, k2, v2, qq), score=256 / 32512 / 12 ** 0.5 * 12 / 128 ** 0.5 if pick else 0.0)
 
 
 @pytest.mark.parametrize('keys', [0, 64, 1000, 10 ** 6])

@@ -226,31 +226,62 @@ __device__ __forceinline__ void store4(u16* o, float4_t v, bool bf16) {
     *gptr((uint2_t*)o) = u;
 }
 
-// 16 query rows (token, head of the group) of one KV head, eight waves that take its blocks in turn. Everything in INT8 MFMAs:
-//   S^T = K Q^T   A = 16 keys x 64 dims as stored, B = the query rows as two INT8 digits each (q = 2^E (256 hi + lo) / 32512, E the
-//                 row's exponent: within 2^-16 of the row's largest value), exact int32 sums;
-//   O^T = V^T P^T A = 16 dims x 64 keys as stored, B = the probabilities of the block as two digits of p / 2^m in 1 / 32639 (m the
-//                 block's own maximum: a block whose probabilities are all small keeps its digits), exact int32 sums.
-// So the cache's bytes are never converted and go from memory straight into the fragments: an FP16 product would spend two instructions
-// on every pair of them. Maximum, sum and outputs are FP32; the scales of a block enter with its exponent's factor (keys) and when its
-// outputs are added (values). The outputs are rescaled only once a maximum is a factor of 256 past the one that they stand on.
-template <int D, int AW>
-__global__ __launch_bounds__(AW * 64, 2) void k_kv8_attend(KvAttend a) {
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+// 16 codes -> two fragments' 8 FP16 values of a lane, exact
+__device__ __forceinline__ void widen(uint4_t w, half8_t& a, half8_t& b) {
+    uint4_t o[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const u32 u = w[k] ^ 0x80808080u;
+        const half2_t off = {(_Float16)1152.f, (_Float16)1152.f};
+        const half2_t x = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+        const half2_t y = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+        o[k >> 1][2 * (k & 1)] = __builtin_bit_cast(u32, x);
+        o[k >> 1][2 * (k & 1) + 1] = __builtin_bit_cast(u32, y);
+    }
+    a = __builtin_bit_cast(half8_t, o[0]);
+    b = __builtin_bit_cast(half8_t, o[1]);
+}
+
+// 16 RT query rows (token, head of the group) of one KV head, W waves that take its blocks in turn. The cache's bytes go from memory straight
+// into MFMA fragments:
+//   S^T = K Q^T   INT8, A = 16 keys x 64 dims as stored, B = the query rows as two digits each (q = 2^E (256 hi + lo) / 32512, E the
+//                 row's exponent: within 2^-16 of the row's largest value), exact int32 sums, so the keys are never converted;
+//   O^T = V^T P^T RT = 1: INT8, A = 16 dims x 64 keys as stored, B = the probabilities of the block as two digits of p / 2^m in 1 / 32639
+//                 (m the block's own maximum: a block whose probabilities are all small keeps its digits), exact int32 sums that are
+//                 scaled and added in FP32: nothing is converted, but every output is touched once a block.
+//                 RT > 1: FP16, A = 16 dims x 32 keys widened in registers (two instructions for two values, for all RT tiles: the byte as
+//                 the low half of 1024 + 128 + code, less 1152, exact), B = the probabilities times the block's value scale / rho, FP32
+//                 sums that stay in the accumulators in units of rho, a power of two near the block's scale (the scale rides on the
+//                 exponent; a unit that changes rescales them exactly, down to 2^-60 of the largest scale so far); the probabilities' sum
+//                 is their product with ones.
+// The outputs are rescaled only once a maximum is a factor of 256 past the one that they stand on.
+// A wave holds one block's keys or values at a time and leaves the overlap of loads, matrix and vector instructions to the other waves of its
+// SIMD (four of them for D up to 128): one wave issues a vector instruction every 7 to 13 cycles here, four together every 3 to 5. With the next
+// block's keys and values already under way (twice the registers, half the waves) 968 causal rows of 16 x 128 took 19.5 us instead of
+// 16.6, 4096 rows 140 instead of 131, and 131000 keys the same 27.5.
+template <int D, int W, int RT>
+__global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_attend(KvAttend a) {
     constexpr int KS = D / 64, DTL = D / 16;
+    constexpr int QN = RT * KS;                                      // (tile, K step) pairs of query digits, one a wave
+    static_assert(QN <= W, "");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
     const int split = blockIdx.x % a.S, tile = blockIdx.x / a.S, h = blockIdx.y, b = blockIdx.z;
     const int c0 = a.cu ? max(0, a.cu[b]) : b * a.most, count = a.cu ? a.cu[b + 1] - c0 : a.most;
     const int m = min(min(count, a.most), a.rows - c0);              // rows computed here
     const int L = min(max(a.lens[b], 0), a.nblk * KB);
-    const int nrows = m * a.G, row0 = 16 * tile;
+    const int nrows = m * a.G, row0 = 16 * RT * tile;
     if (row0 >= nrows) return;                                       // uniform
-    const int r = row0 + lr, t = r / a.G, hq = h * a.G + (r - t * a.G);
-    const bool on = r < nrows;
     auto sees = [&](int tt) { return a.causal ? min(max(L - count + tt + 1, 0), L) : L; };
-    const int vend = on ? sees(t) : 0, all = __builtin_amdgcn_readfirstlane(sees(row0 / a.G));
-    const int kend = __builtin_amdgcn_readfirstlane(sees((min(row0 + 16, nrows) - 1) / a.G));
-    const int nb = (kend + KB - 1) / KB, step = AW * a.S;
+    auto token = [&](int r, int& hq) {                               // row r of the KV head: its token and query head
+        const int t = r / a.G;
+        hq = h * a.G + (r - t * a.G);
+        return t;
+    };
+    const int all = __builtin_amdgcn_readfirstlane(sees(row0 / a.G));
+    const int kend = __builtin_amdgcn_readfirstlane(sees((min(row0 + 16 * RT, nrows) - 1) / a.G));
+    const int nb = (kend + KB - 1) / KB, step = W * a.S;
     const size_t bh = (size_t)b * a.Hk + h;
     const i8* kb = a.k8 + bh * a.nblk * (size_t)(KB * D);
     const i8* vb = a.v8 + bh * a.nblk * (size_t)(KB * D);
@@ -271,57 +302,67 @@ __global__ __launch_bounds__(AW * 64, 2) void k_kv8_attend(KvAttend a) {
 #pragma unroll
         for (int dt = 0; dt < DTL; ++dt) V[dt] = *gptr((const uint4_t*)(p + dt * 1024 + lane * 16));
     };
-    constexpr bool EARLY = D < 256;                                  // whether the values of the next block are fetched while this one's wait
-    int j = split * AW + wave;
-    // the query row's digits: wave ks < KS makes K step ks, this lane's dims 64 ks + 16 lg .. + 15, after the waves' maxima have met in LDS
-    uint4_t w0 = {0, 0, 0, 0}, w1 = {0, 0, 0, 0};
-    if (wave < KS) {
-        const u16* qp = a.q + (c0 + (int64_t)(on ? t : 0)) * a.q_tok + (int64_t)(on ? hq : h * a.G) * a.q_head + 16 * lg + 64 * wave;
-        w0 = gptr((const uint4_t*)qp)[0];
-        w1 = gptr((const uint4_t*)qp)[1];
+    int j = split * W + wave;
+    // the query rows' digits: wave KS rt + ks makes K step ks of tile rt, this lane's dims 64 ks + 16 lg .. + 15 of row lr, after the
+    // maxima have met in LDS
+    uint4_t wq[2];
+    const int qt = wave / KS;
+    if (wave < QN) {
+        const int r = row0 + 16 * qt + lr;
+        int hq;
+        const int t = token(r < nrows ? r : 0, hq);                  // (rows past the last one read the first)
+        const u16* at = a.q + (c0 + (int64_t)t) * a.q_tok + (int64_t)hq * a.q_head + 16 * lg + 64 * (wave - KS * qt);
+        wq[0] = gptr((const uint4_t*)at)[0];
+        wq[1] = gptr((const uint4_t*)at)[1];
     }
-    if (j < nb) {
-        load_k(j);
-        if (EARLY) load_v(j);
-    }
-    auto local_barrier = [] {                                        // (the loads in flight go on)
+    auto local_barrier = [] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     };
-    float* const qmax = (float*)(lds + KS * 2048);
-    float v[16], mq = 0.f, qbad = 0.f;
-    if (wave < KS) {
+    float* const qmax = (float*)(lds + QN * 2048);
+    auto value = [&](int x) { return kv_value((u16)(wq[x >> 3][(x >> 1) & 3] >> (16 * (x & 1))), a.bf16); };
+    if (wave < QN) {
+        float mq = 0.f, bad = 0.f;
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-            v[x] = kv_value((u16)((x < 8 ? w0 : w1)[(x >> 1) & 3] >> (16 * (x & 1))), a.bf16);
-            mq = fmaxf(mq, fabsf(v[x]));
-            qbad = __builtin_fmaf(v[x], 0.f, qbad);                  // NaN once a value is not finite
+            mq = fmaxf(mq, fabsf(value(x)));
+            bad = __builtin_fmaf(value(x), 0.f, bad);                // NaN once a value is not finite
         }
         mq = fmaxf(mq, lane_xor(mq, 16, lane));
         mq = fmaxf(mq, lane_xor(mq, 32, lane));
-        qbad += lane_xor(qbad, 16, lane);
-        qbad += lane_xor(qbad, 32, lane);
-        if (lg == 0) qmax[16 * wave + lr] = qbad != 0.f ? qbad : mq;
+        bad += lane_xor(bad, 16, lane);
+        bad += lane_xor(bad, 32, lane);
+        if (lg == 0) qmax[16 * wave + lr] = bad != 0.f ? bad : mq;
     }
     local_barrier();
-    mq = 0.f;
-    qbad = 0.f;
+    int E[RT], vend[RT];
+    float qs[RT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-        const float x = qmax[16 * ks + lr];
-        mq = fmaxf(mq, x);
-        qbad = __builtin_isnan(x) ? x : qbad;
+    for (int rt = 0; rt < RT; ++rt) {
+        float mq = 0.f, bad = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const float x = qmax[16 * (KS * rt + ks) + lr];
+            mq = fmaxf(mq, x);
+            bad = __builtin_isnan(x) ? x : bad;
+        }
+        if (bad != 0.f) mq = 1.f;                                    // the row's scores become NaN below
+        E[rt] = mq > 0.f ? __builtin_amdgcn_frexp_expf(mq) : 0;
+        qs[rt] = a.sl / QC + bad;
+        const int r = row0 + 16 * rt + lr;
+        vend[rt] = r < nrows ? sees(r / a.G) : 0;
     }
-    if (qbad != 0.f) mq = 1.f;                                       // the row's scores become NaN below
-    const int E = mq > 0.f ? __builtin_amdgcn_frexp_expf(mq) : 0;
-    if (wave < KS) {
+    if (wave < QN) {
+        int e = E[0];
+#pragma unroll
+        for (int rt = 1; rt < RT; ++rt) e = qt == rt ? E[rt] : e;
         uint4_t dh, dl;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             float f[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) f[y] = __builtin_fmaf(__builtin_amdgcn_ldexpf(v[4 * x + y], -E), QC, DIG);
+            for (int y = 0; y < 4; ++y) f[y] = __builtin_fmaf(__builtin_amdgcn_ldexpf(value(4 * x + y), -e), QC, DIG);
             u32 hi, lo;
             digits(f[0], f[1], f[2], f[3], hi, lo);
             dh[x] = hi;
@@ -331,127 +372,204 @@ __global__ __launch_bounds__(AW * 64, 2) void k_kv8_attend(KvAttend a) {
         ((uint4_t*)lds)[(2 * wave + 1) * 64 + lane] = dl;
     }
     local_barrier();
-    const float qs = a.sl / QC + qbad;
-    const uint4_t* Q = (const uint4_t*)lds + lane;                   // digits hi, lo of K step ks at 128 ks, 128 ks + 64
-    float4_t O[DTL];
+    const uint4_t* Q = (const uint4_t*)lds + lane;                   // digits hi, lo of K step ks of tile rt at 128 (KS rt + ks), + 64
+    float4_t O[RT][DTL];
+    float mr[RT], l[RT], top = 0.f;
+    int er = -126;                                                   // RT > 1: rho = 2^er
 #pragma unroll
-    for (int dt = 0; dt < DTL; ++dt) O[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-    float mr = -__builtin_inff(), l = 0.f;
+    for (int rt = 0; rt < RT; ++rt) {
+        mr[rt] = -__builtin_inff();
+        l[rt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DTL; ++dt) O[rt][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
     auto block = [&](auto edge) {
-        const bool more = j + step < nb;
-        const float c = __builtin_amdgcn_ldexpf(qs * sk, E), svc = sv * (1.f / PC);
-        float f[16];
-        int4_t hi[4], lo[4];
+        load_k(j);
+        float c[RT], f[RT][16];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const uint4_t qh = Q[128 * ks], ql = Q[128 * ks + 64];
+        for (int rt = 0; rt < RT; ++rt) {
+            c[rt] = __builtin_amdgcn_ldexpf(qs[rt] * sk, E[rt]);
+            int4_t hi[4], lo[4];
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                hi[kt] = mma_i8(K[kt][ks], qh, ks ? hi[kt] : int4_t{0, 0, 0, 0});
-                lo[kt] = mma_i8(K[kt][ks], ql, ks ? lo[kt] : int4_t{0, 0, 0, 0});
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint4_t qh = Q[128 * (KS * rt + ks)], ql = Q[128 * (KS * rt + ks) + 64];
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt) {
+                    hi[kt] = mma_i8(K[kt][ks], qh, ks ? hi[kt] : int4_t{0, 0, 0, 0});
+                    lo[kt] = mma_i8(K[kt][ks], ql, ks ? lo[kt] : int4_t{0, 0, 0, 0});
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 16; ++x) f[rt][x] = (float)((hi[x >> 2][x & 3] << 8) + lo[x >> 2][x & 3]);
+        }
+        __builtin_amdgcn_sched_barrier(0);                           // (the values' loads no earlier: they take the keys' registers)
+        load_v(j);
+        auto left = [&](int rt, int x) { return 16 * (x >> 2) + (x & 3) < vend[rt] - j * KB - 4 * lg; };   // key x of this lane group is visible
+        auto largest = [&](int rt) {
+            if constexpr (edge)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) f[rt][x] = left(rt, x) ? f[rt][x] : -__builtin_inff();
+            float mx = f[rt][0];
+#pragma unroll
+            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, f[rt][x]);
+            return mx;
+        };
+        auto across = [&](float mx) {
+            mx = fmaxf(mx, lane_xor(mx, 16, lane));
+            return fmaxf(mx, lane_xor(mx, 32, lane));
+        };
+        if constexpr (RT == 1) {
+            const float mx = across(largest(0));
+            const bool none = edge && mx == -__builtin_inff();       // the row sees no key of the block
+            const float mb = none ? 0.f : mx * c[0];
+            float p[16], lb = 0.f;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[0][x], c[0], -mb));
+            if constexpr (edge)                                      // also where c is 0 and the product above NaN
+#pragma unroll
+                for (int x = 0; x < 16; ++x) p[x] = left(0, x) ? p[x] : 0.f;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) lb += p[x];
+            uint4_t Ph, Pl;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                u32 h4, l4;
+                digits(__builtin_fmaf(p[4 * x], PC, DIG), __builtin_fmaf(p[4 * x + 1], PC, DIG), __builtin_fmaf(p[4 * x + 2], PC, DIG),
+                       __builtin_fmaf(p[4 * x + 3], PC, DIG), h4, l4);
+                Ph[x] = h4;
+                Pl[x] = l4;
+            }
+            const bool up = !none && mb > mr[0] + 8.f;
+            if (__builtin_amdgcn_ballot_w64(up)) {                   // uniform
+                const float al = up ? __builtin_amdgcn_exp2f(mr[0] - mb) : 1.f;
+                l[0] *= al;
+#pragma unroll
+                for (int dt = 0; dt < DTL; ++dt) O[0][dt] *= al;
+                mr[0] = up ? mb : mr[0];
+            }
+            const float w = none ? 0.f : __builtin_amdgcn_exp2f(mb - mr[0]), be = none ? 0.f : w * (sv * (1.f / PC));
+            l[0] = __builtin_fmaf(w, lb, l[0]);
+#pragma unroll
+            for (int dt = 0; dt < DTL; ++dt) {
+                const int4_t z = {0, 0, 0, 0};
+                const int4_t oh = mma_i8(V[dt], Ph, z), ol = mma_i8(V[dt], Pl, z);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) O[0][dt][e] = __builtin_fmaf((float)((oh[e] << 8) + ol[e]), be, O[0][dt][e]);
+            }
+        } else {
+            // the unit of the outputs, changed when the scale leaves [unit / 64, unit]
+            int shift = 0;
+            const int es = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(sv));
+            if (es > er || es < er - 6) {                            // uniform
+                top = fmaxf(top, sv);
+                const int ne = max(min(es, 127), __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) - 60);
+                shift = er - ne;
+                er = ne;
+            }
+            // p sv = 2^(s - m + lu) rho; their sum in units of the probabilities is iu times what the MFMA adds
+            const float lu = __builtin_amdgcn_logf(sv) - (float)er, iu = __builtin_amdgcn_exp2f(-lu);
+            half8_t P[RT][2], ones;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) ones[x] = (_Float16)1.f;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float mx = largest(rt);
+                if (shift || __builtin_amdgcn_ballot_w64(mx * c[rt] > mr[rt] + 8.f)) {   // uniform
+                    mx = across(mx);
+                    const float mb = edge && mx == -__builtin_inff() ? mx : mx * c[rt];
+                    const bool up = mb > mr[rt] + 8.f;
+                    const float al = up ? __builtin_amdgcn_exp2f(mr[rt] - mb) : 1.f, ak = __builtin_amdgcn_ldexpf(al, shift);
+                    l[rt] *= al;
+#pragma unroll
+                    for (int dt = 0; dt < DTL; ++dt) O[rt][dt] *= ak;
+                    mr[rt] = up ? mb : mr[rt];
+                }
+                const float mz = edge && mr[rt] == -__builtin_inff() ? 0.f : mr[rt] - lu;
+                float p[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[rt][x], c[rt], -mz));
+                if constexpr (edge)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) p[x] = left(rt, x) ? p[x] : 0.f;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) P[rt][x >> 3][x & 7] = (_Float16)p[x];
+                float4_t s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[rt][0], float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[rt][1], s, 0, 0, 0);
+                l[rt] = __builtin_fmaf(s[0], iu, l[rt]);             // (the same in all four lane groups)
+            }
+#pragma unroll
+            for (int dt = 0; dt < DTL; ++dt) {
+                half8_t A[2];
+                widen(V[dt], A[0], A[1]);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) O[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[s], P[rt][s], O[rt][dt], 0, 0, 0);
             }
         }
-#pragma unroll
-        for (int x = 0; x < 16; ++x) f[x] = (float)((hi[x >> 2][x & 3] << 8) + lo[x >> 2][x & 3]);
-        if (!EARLY) {                                                // keys and values share what registers D = 256 leaves
-            __builtin_amdgcn_sched_barrier(0);
-            load_v(j);
-        }
-        if (more) load_k(j + step);
-        const int left = vend - j * KB - 4 * lg;                     // key 16 (x / 4) + x % 4 of this lane group is visible below it
-        if constexpr (edge)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) f[x] = 16 * (x >> 2) + (x & 3) < left ? f[x] : -__builtin_inff();
-        float mx = f[0];
-#pragma unroll
-        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, f[x]);
-        mx = fmaxf(mx, lane_xor(mx, 16, lane));
-        mx = fmaxf(mx, lane_xor(mx, 32, lane));
-        const bool none = edge && mx == -__builtin_inff();           // the row sees no key of the block
-        const float mb = none ? 0.f : mx * c;
-        float p[16], lb = 0.f;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[x], c, -mb));
-        if constexpr (edge)                                          // also where c is 0 and the product above NaN
-#pragma unroll
-            for (int x = 0; x < 16; ++x) p[x] = 16 * (x >> 2) + (x & 3) < left ? p[x] : 0.f;
-#pragma unroll
-        for (int x = 0; x < 16; ++x) lb += p[x];
-        uint4_t Ph, Pl;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            u32 h4, l4;
-            digits(__builtin_fmaf(p[4 * x], PC, DIG), __builtin_fmaf(p[4 * x + 1], PC, DIG), __builtin_fmaf(p[4 * x + 2], PC, DIG),
-                   __builtin_fmaf(p[4 * x + 3], PC, DIG), h4, l4);
-            Ph[x] = h4;
-            Pl[x] = l4;
-        }
-        const bool up = !none && mb > mr + 8.f;
-        if (__builtin_amdgcn_ballot_w64(up)) {                       // uniform
-            const float al = up ? __builtin_amdgcn_exp2f(mr - mb) : 1.f;
-            l *= al;
-#pragma unroll
-            for (int dt = 0; dt < DTL; ++dt) O[dt] *= al;
-            mr = up ? mb : mr;
-        }
-        const float w = none ? 0.f : __builtin_amdgcn_exp2f(mb - mr), be = none ? 0.f : w * svc;
-        l = __builtin_fmaf(w, lb, l);
-#pragma unroll
-        for (int dt = 0; dt < DTL; ++dt) {
-            const int4_t z = {0, 0, 0, 0};
-            const int4_t oh = mma_i8(V[dt], Ph, z), ol = mma_i8(V[dt], Pl, z);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[dt][e] = __builtin_fmaf((float)((oh[e] << 8) + ol[e]), be, O[dt][e]);
-        }
-        if (EARLY && more) load_v(j + step);
         j += step;
     };
     const int whole = all / KB;                                      // blocks that every row sees whole (rows past the last one do not count)
     while (j < min(nb, whole)) block(std::false_type());
     while (j < nb) block(std::true_type());
-    // merge the waves through LDS: statistics and outputs, wave w summing its share of the dims
+    // merge the waves through LDS: statistics and outputs, wave w summing its share of the dim tiles
     __syncthreads();
-    constexpr int WD = DTL < AW ? DTL : AW, DW = DTL / WD;           // waves that sum, dim tiles of each
+    constexpr int NT = RT * DTL, WD = NT < W ? NT : W, DW = NT / WD; // dim tiles, waves that sum, dim tiles of each
     float4_t* x = (float4_t*)lds;
-    float *sm = (float*)(lds + AW * DTL * 1024), *sl = sm + 16 * AW;
-    l += lane_xor(l, 16, lane);
-    l += lane_xor(l, 32, lane);
-    if (lg == 0) {
-        sm[16 * wave + lr] = mr;
-        sl[16 * wave + lr] = l;
-    }
+    float *sm = (float*)(lds + W * NT * 1024), *sl = sm + 16 * RT * W;
+    const float rho = RT == 1 ? 1.f : __builtin_amdgcn_ldexpf(1.f, er);
 #pragma unroll
-    for (int dt = 0; dt < DTL; ++dt) x[(wave * DTL + dt) * 64 + lane] = O[dt];
-    __syncthreads();
-    if (wave >= WD || !on) return;
-    float mx = -__builtin_inff(), lsum = 0.f, wt[AW];
-#pragma unroll
-    for (int w = 0; w < AW; ++w) mx = fmaxf(mx, sm[16 * w + lr]);
-#pragma unroll
-    for (int w = 0; w < AW; ++w) {
-        // a wave without a visible key has l = 0 and weight 0; one whose scores are NaN has l = NaN and weight NaN
-        const float mw = sm[16 * w + lr], lw = sl[16 * w + lr];
-        wt[w] = mw == -__builtin_inff() ? lw : __builtin_amdgcn_exp2f(mw - mx);
-        lsum = __builtin_fmaf(wt[w], lw, lsum);
-    }
-    const size_t row = (size_t)(c0 + t) * (a.Hk * a.G) + hq;
-    if (a.S > 1 && wave == 0 && lg == 0) {
-        a.stat[(row * a.S + split) * 2] = mx;
-        a.stat[(row * a.S + split) * 2 + 1] = lsum;
-    }
-    const float inv = lsum == 0.f ? 0.f : 1.f / lsum;                // a row that sees no key: zeros
-#pragma unroll
-    for (int k = 0; k < DW; ++k) {
-        const int dt = wave * DW + k;
-        float4_t s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < AW; ++w) {
-            const float4_t v = x[(w * DTL + dt) * 64 + lane];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(wt[w], v[e], s[e]);
+    for (int rt = 0; rt < RT; ++rt) {
+        float s = l[rt];
+        if (RT == 1) {
+            s += lane_xor(s, 16, lane);
+            s += lane_xor(s, 32, lane);
         }
-        if (a.S > 1) *gptr((float4_t*)(a.part + (row * a.S + split) * D + 16 * dt + 4 * lg)) = s;
-        else store4(a.o + row * D + 16 * dt + 4 * lg, s * inv, a.bf16);
+        if (lg == 0) {
+            sm[16 * (RT * wave + rt) + lr] = mr[rt];
+            sl[16 * (RT * wave + rt) + lr] = s;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DTL; ++dt) x[(wave * NT + rt * DTL + dt) * 64 + lane] = RT == 1 ? O[rt][dt] : O[rt][dt] * rho;
+    }
+    __syncthreads();
+    if (wave >= WD) return;
+    constexpr int TW = DW < DTL ? 1 : DW / DTL, TD = DW / TW;        // row tiles that a wave sums, dim tiles of each
+#pragma unroll
+    for (int i = 0; i < TW; ++i) {
+        const int rt = TW > 1 ? wave * TW + i : wave * DW / DTL, d0 = TW > 1 ? 0 : wave * DW % DTL, r = row0 + 16 * rt + lr;
+        if (r >= nrows) continue;
+        float mx = -__builtin_inff(), lsum = 0.f, wt[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, sm[16 * (RT * w + rt) + lr]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            // a wave without a visible key has l = 0 and weight 0; one whose scores are NaN has l = NaN and weight NaN
+            const float mw = sm[16 * (RT * w + rt) + lr], lw = sl[16 * (RT * w + rt) + lr];
+            wt[w] = mw == -__builtin_inff() ? lw : __builtin_amdgcn_exp2f(mw - mx);
+            lsum = __builtin_fmaf(wt[w], lw, lsum);
+        }
+        int hq;
+        const int t = token(r, hq);
+        const size_t row = (size_t)(c0 + t) * (a.Hk * a.G) + hq;
+        if (a.S > 1 && d0 == 0 && lg == 0) {
+            a.stat[(row * a.S + split) * 2] = mx;
+            a.stat[(row * a.S + split) * 2 + 1] = lsum;
+        }
+        const float inv = lsum == 0.f ? 0.f : 1.f / lsum;            // a row that sees no key: zeros
+#pragma unroll
+        for (int k = 0; k < TD; ++k) {
+            const int dt = d0 + k;
+            float4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float4_t y = x[(w * NT + rt * DTL + dt) * 64 + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(wt[w], y[e], s[e]);
+            }
+            if (a.S > 1) *gptr((float4_t*)(a.part + (row * a.S + split) * D + 16 * dt + 4 * lg)) = s;
+            else store4(a.o + row * D + 16 * dt + 4 * lg, s * inv, a.bf16);
+        }
     }
 }
 
@@ -546,24 +664,31 @@ __global__ __launch_bounds__(KT) void k_kv8_join(KvAttend a) {
     store4(a.o + row * D + 4 * d, acc * (tot == 0.f ? 0.f : 1.f / tot), a.bf16);
 }
 
-size_t kv_attend_lds(int D, int W) { return (size_t)W * (D / 16) * 1024 + W * 128; }   // the waves' outputs and statistics (over the digits)
+size_t kv_attend_lds(int D, int W, int RT) {     // the waves' outputs and statistics, or the query digits and maxima before them
+    return max((size_t)W * RT * ((D / 16) * 1024 + 128), (size_t)RT * (D / 64) * (2048 + 64));
+}
 bool kv_dim(int D) { return D == 64 || D == 128 || D == 256; }
 bool kv_size(int B, int H, int nblk) { return B > 65535 || H > 65535 || nblk > (1 << 25) - 1; }
 
-// How a call is split: the waves W of a workgroup, which take the blocks of 16 rows of a KV head in turn, and the parts S of their keys.
-// Few rows over up to 16 blocks: one launch of eight waves (968 keys of one sequence, D = 256: 10.5 us against 8.8 in parts of four waves with
-// their join, but a call from Python 12.5 us against 16.4). Else four waves, two workgroups a CU (968 causal rows of 8 heads 17 us, with
-// eight waves 20), in as many parts as give every CU one of them. Where that is fewer than 4 and the parts stay long, up to two a CU: the
-// lengths of a batch differ (16 sequences of 4 to 8 thousand keys, 8 heads of 128: 48 us against 54; of 3 thousand, 64 dims: 22 against 19).
+// How a call is split: the waves W of a workgroup, which take the blocks of 16 RT rows of a KV head in turn, and the parts S of their keys.
+//   Two tiles of 16 rows a wave (D = 128) where that still makes two workgroups a CU: 1024 rows behind 4096 keys, 2 sequences of 16 x 8 heads
+//   99 us against 111, 300 rows behind 1000 16.5 against 13.7. (D = 64: 42 us against 36 at 4 x 1024 rows. D = 256: its registers.)
+//   Few rows over up to 16 blocks: one launch of eight waves (968 keys of one sequence, D = 256: 10.5 us against 8.8 in parts of four waves
+//   with their join, but a call from Python 12 us against 16).
+//   Else four waves (968 causal rows of 8 heads x 256 16 us, with eight 20), in as many parts as give every CU a workgroup. Where that is
+//   fewer than 4 and the parts stay long, as many as fit: the lengths of a batch differ (16 sequences of 4 to 8 thousand keys, 8 heads of
+//   128: 47 us against 54; of 1.5 to 3 thousand, 64 dims, 22 against 19).
 struct KvPlan {
-    int W, S;
+    int W, S, RT;
 };
 KvPlan kv_plan(int B, int most, int G, int Hk, int D, int keys) {
-    const int64_t groups = (int64_t)B * Hk * (((int64_t)most * G + 15) / 16), nb = ((int64_t)keys + KB - 1) / KB;
-    if (groups <= 256 && nb <= 16) return {8, 1};
+    const int64_t n = (int64_t)most * G, heads = (int64_t)B * Hk, nb = ((int64_t)keys + KB - 1) / KB;
+    if (D == 128 && heads * ((n + 31) / 32) >= 512) return {4, 1, 2};
+    const int64_t groups = heads * ((n + 15) / 16);
+    if (groups <= 256 && nb <= 16) return {8, 1, 1};
     int64_t S = max((int64_t)1, min(256 / groups, (nb + 3) / 4));
-    if (S < 4) S = max(S, min(512 / groups, nb * D / 2048));
-    return {4, (int)min(S, (int64_t)MAX_SPLITS)};
+    if (S < 4) S = max(S, min((D == 256 ? 512 : 1024) / groups, nb * D / 2048));
+    return {4, (int)min(S, (int64_t)MAX_SPLITS), 1};
 }
 
 }  // namespace
@@ -632,7 +757,7 @@ extern "C" int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int 
     const int G = Hq / Hk;
     const KvPlan plan = kv_plan(B, most, G, Hk, D, keys);
     const int S = plan.S;
-    const int64_t tiles = ((int64_t)most * G + 15) / 16;
+    const int64_t tiles = ((int64_t)most * G + 16 * plan.RT - 1) / (16 * plan.RT);
     if (tiles * S > 0x7fffffff || (int64_t)most * Hq > 0x7fffffff || (int64_t)rows * Hq > 0x7fffffff) return TCQ_ERR_UNSUPPORTED;
     if (S > 1 && !part) return TCQ_ERR_ARG;
     if (((uintptr_t)q | (uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)o | (uintptr_t)part) % 16 || (q_tok | q_head) % 8 || (uintptr_t)scale % 8)
@@ -643,14 +768,16 @@ extern "C" int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int 
 #define KV_ATTEND(N)                                                                                                    \
     do {                                                                                                                \
         const dim3 grid((u32)(tiles * S), Hk, B);                                                                       \
-        if (plan.W == 8) launch_k(k_kv8_attend<N, 8>, grid, dim3(512), kv_attend_lds(N, 8), st, a);                     \
-        else launch_k(k_kv8_attend<N, 4>, grid, dim3(256), kv_attend_lds(N, 4), st, a);                                 \
+        const size_t lds = kv_attend_lds(N, plan.W, plan.RT);                                                           \
+        if (plan.W == 8) launch_k(k_kv8_attend<N, 8, 1>, grid, dim3(512), lds, st, a);                                  \
+        else if (N != 128 || plan.RT == 1) launch_k(k_kv8_attend<N, 4, 1>, grid, dim3(256), lds, st, a);                \
+        else launch_k(k_kv8_attend<128, 4, 2>, grid, dim3(256), lds, st, a);                                            \
         if (S > 1) {                                                                                                    \
             const int e = launch_status();                                                                              \
             if (e) return e;                                                                                            \
-            constexpr int R = KT / (N / 4);                                                                             \
+            constexpr int PR = KT / (N / 4);                                                                            \
             if (S > 8) launch_k(k_kv8_join<N>, dim3((u32)most * Hq, 1, B), dim3(KT), 0, st, a);                         \
-            else launch_k(k_kv8_join_few<N>, dim3(((u32)most * Hq + R - 1) / R, 1, B), dim3(KT), 0, st, a);             \
+            else launch_k(k_kv8_join_few<N>, dim3(((u32)most * Hq + PR - 1) / PR, 1, B), dim3(KT), 0, st, a);             \
         }                                                                                                               \
     } while (0)
     KV_BY_DIM(KV_ATTEND);
