@@ -326,8 +326,8 @@ int tcq_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int
  * head strides in elements, go to positions start[b], start[b] + 1, ... What a sequence held from start[b] on is gone; the rows
  * before it in start[b]'s block come from the tail, so start[b] lies at most one whole block before the newest block written
  * (an append that ended at start[b], or one that is taken back by up to 64 rows). Every touched block is quantized anew from its 16-bit
- * rows, so a block's codes depend on its rows alone. Rows past the capacity, past `most` of a sequence or past `rows` are dropped;
- * a sequence without new rows is left as it is. */
+ * rows, so a block's codes depend on its rows alone. Rows past the capacity, past `most` of a sequence or past `rows` are dropped, a
+ * negative start counts as 0; a sequence without new rows is left as it is. */
 int tcq_kv8_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int dtype, const int32_t* cu,
                    const int32_t* start, int rows, int most, int B, int H, int D, int nblk, int8_t* k8, int8_t* v8, float* scale, void* tail,
                    tcq_stream_t stream);
@@ -342,7 +342,7 @@ int tcq_kv8_read(const int8_t* k8, const int8_t* v8, const float* scale, const i
  * sequence has (it sets how far the work is split, never the result's meaning). part: workspace of tcq_kv8_attend_floats(...) floats,
  * 16-byte aligned (NULL where that is 0), not shared by calls that overlap. Scores from the query as 16-bit integers (within 2^-16 of the
  * row's largest value) and the probabilities as 16-bit integers of their block's maximum, exact int32 products with the codes, FP32
- * maximum, sum and outputs. */
+ * maximum, sum and outputs (many rows of D = 128: FP16 probabilities of the running maximum instead). */
 int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, const int32_t* lens, int rows, int most, int B,
                    int Hq, int Hk, int D, int nblk, const int8_t* k8, const int8_t* v8, const float* scale, int causal, float score_scale,
                    int keys, float* part, void* o, tcq_stream_t stream);

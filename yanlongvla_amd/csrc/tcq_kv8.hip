@@ -15,7 +15,7 @@ struct KvAppend {
     i8 *k8, *v8;
     float* scale;
     u16* tail;
-    int rows, most, H, D, nblk;
+    int rows, most, H, D, nblk, near;
 };
 
 // A value as the cache holds it: NaN as 0, an infinity as the block's largest code; 8 bits have neither.
@@ -32,6 +32,8 @@ __device__ __forceinline__ float kv_mag(float v) {
 // bits of two values at a time; only a block where that is no finite number looks at each value.
 // The rows of the newest two blocks go to the tail. Where that overwrites the rows that the first block reads (a newest block of its
 // parity), the first block's workgroup writes them, after its reads.
+// MI355X: 4500 rows of 6 prompts, 8 heads of 128 11.5 us (28 MB: 2.4 TB/s; instruction issue, 14 us before whole blocks had one base address and
+// 36 with 32 values a thread, a load waiting for each row's branch); one row each of 16 sequences, one head of 256, 7.2 us (latency).
 template <int D, bool BF, bool VEC>
 __global__ __launch_bounds__(4 * D) void k_kv8_append(KvAppend a) {
     __shared__ float red[16];
@@ -52,14 +54,32 @@ __global__ __launch_bounds__(4 * D) void k_kv8_append(KvAppend a) {
     u32 raw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     // keys: dims d .. d + 15 of token t; values: tokens 16 (x / 4) + t + x % 4 of dim d, t = 4 lane group
     const int t = val ? tid / D * 4 : (tid & 15) + 16 * (tid / D), d = val ? tid % D : (tid >> 4) % (D / 16) * 16;
-    // (a row past the last one reads that one, so that no load waits for a branch, and counts as zeros)
-    if (!val) {
+    u16 x[16];
+    if (p0 >= s && p0 + KB <= e && a.near) {                   // uniform: a whole block of the call's rows, one base and 32-bit offsets
+        const u16* base = in + (int64_t)p0 * tok;
+        const u32 off = (u32)t * (u32)tok + (u32)d;
+        if (val) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = gptr(base + (int64_t)(16 * (i >> 2) + (i & 3)) * tok)[off];
+        } else if (VEC) {
+            const uint4_t y = gptr((const uint4_t*)(base + off))[0], z = gptr((const uint4_t*)(base + off))[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i] = y[i], raw[4 + i] = z[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = gptr(base + off)[i];
+        }
+        if (val || !VEC)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) raw[i] = (u32)x[2 * i] | ((u32)x[2 * i + 1] << 16);
+    } else if (!val) {
+        // (a row past the last one reads that one, so that no load waits for a branch, and counts as zeros)
         const int p = p0 + t;
         const u16* r = (p < s ? slot + t * D : in + (int64_t)min(p, e - 1) * tok) + d;
         if (VEC) {
-            const uint4_t x = gptr((const uint4_t*)r)[0], y = gptr((const uint4_t*)r)[1];
+            const uint4_t y = gptr((const uint4_t*)r)[0], z = gptr((const uint4_t*)r)[1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[i] = x[i], raw[4 + i] = y[i];
+            for (int i = 0; i < 4; ++i) raw[i] = y[i], raw[4 + i] = z[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) raw[i >> 1] |= (u32)gptr(r)[i] << (16 * (i & 1));
@@ -67,7 +87,6 @@ __global__ __launch_bounds__(4 * D) void k_kv8_append(KvAppend a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[i] = p < e ? raw[i] : 0;
     } else {
-        u16 x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int key = 16 * (i >> 2) + t + (i & 3), p = p0 + key;
@@ -135,10 +154,12 @@ struct KvRead {
     int n, H, D, nblk, dt;
 };
 
-__device__ __forceinline__ u32 kv_pair(float x, float y, int dt) { return dt == TCQ_BF16 ? bf16x2(x, y) : (u32)f32_to_f16(x) | ((u32)f32_to_f16(y) << 16); }
+__device__ __forceinline__ u32 kv_pair(float x, float y, int dt) {   // (finite values)
+    return dt == TCQ_BF16 ? bf16_cvt2(x, y) : (u32)f32_to_f16(x) | ((u32)f32_to_f16(y) << 16);
+}
 
 // grid (2 x D / 64 x blocks a window may touch, H, B): 256 pieces of 16 values of a block's keys (even block index) or values; k, v (B, n, H, D),
-// row i of sequence b is position first[b] + i, zeros from lens[b] on.
+// row i of sequence b is position first[b] + i, zeros from lens[b] on. MI355X: 6 x 1024 rows, 8 heads of 128 11.7 us (38 MB, 3.2 TB/s).
 template <int D>
 __global__ __launch_bounds__(KT) void k_kv8_read(KvRead a) {
     const int b = blockIdx.z, h = blockIdx.y, bx = blockIdx.x / (D / 64), val = bx & 1, u = blockIdx.x % (D / 64) * KT + threadIdx.x;
@@ -148,46 +169,48 @@ __global__ __launch_bounds__(KT) void k_kv8_read(KvRead a) {
     const bool there = blk < a.nblk;
     const size_t at = ((size_t)b * a.H + h) * a.nblk + (there ? blk : 0);
     const int es = a.dt == TCQ_F32 ? 4 : 2;
-    const int64_t i0 = p0 - first, row = (int64_t)a.H * D * es;                      // row of token 0; bytes from row to row
-    char* const out = (val ? a.v : a.k) + ((int64_t)b * a.n * a.H + h) * D * es + i0 * row;
+    const int lo = (int)max((int64_t)0, first - p0), hi = (int)min((int64_t)KB, first + (int64_t)a.n - p0);   // tokens of the block in the window,
+    const int have = (int)max((int64_t)0, min((int64_t)KB, end - p0));                                       // and those that it holds
+    const size_t row = (size_t)a.H * D * es;                                         // bytes from row to row
+    char* const out = (val ? a.v : a.k) + ((int64_t)b * a.n + (p0 - first)) * (int64_t)row + (size_t)h * D * es;
     const float sc = there ? a.scale[at * 2 + val] : 0.f;
     const i8* in = (val ? a.v8 : a.k8) + at * (size_t)(KB * D);
     if (!val) {
         const int key = (u & 15) + 16 * (u / D), d = (u >> 4) % (D / 16) * 16;
-        if (i0 + key < 0 || i0 + key >= a.n) return;
+        if (key < lo || key >= hi) return;
         uint4_t w = {0, 0, 0, 0};
-        if (p0 + key < end) w = *gptr((const uint4_t*)(in + (size_t)u * 16));
+        if (key < have) w = *gptr((const uint4_t*)(in + (size_t)u * 16));
         float v[16];
 #pragma unroll
-        for (int x = 0; x < 16; ++x) v[x] = (float)(i8)(w[x >> 2] >> (8 * (x & 3))) * sc;
-        uint4_t* q = (uint4_t*)(out + key * row + (size_t)d * es);
+        for (int x = 0; x < 16; ++x) v[x] = i8_f32(w[x >> 2], x & 3) * sc;
+        if (key >= have)                                                             // (a block that nothing was written to has any scale)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            if (a.dt == TCQ_F32)
+            for (int x = 0; x < 16; ++x) v[x] = 0.f;
+        uint4_t* q = (uint4_t*)(out + key * row + (size_t)d * es);
+        if (a.dt == TCQ_F32) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
                 gptr(q)[x] = uint4_t{__float_as_uint(v[4 * x]), __float_as_uint(v[4 * x + 1]), __float_as_uint(v[4 * x + 2]), __float_as_uint(v[4 * x + 3])};
-            else if (!(x & 1))
-                gptr(q)[x >> 1] = uint4_t{kv_pair(v[4 * x], v[4 * x + 1], a.dt), kv_pair(v[4 * x + 2], v[4 * x + 3], a.dt),
-                                          kv_pair(v[4 * x + 4], v[4 * x + 5], a.dt), kv_pair(v[4 * x + 6], v[4 * x + 7], a.dt)};
+        } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                gptr(q)[x] = uint4_t{kv_pair(v[8 * x], v[8 * x + 1], a.dt), kv_pair(v[8 * x + 2], v[8 * x + 3], a.dt),
+                                     kv_pair(v[8 * x + 4], v[8 * x + 5], a.dt), kv_pair(v[8 * x + 6], v[8 * x + 7], a.dt)};
         }
     } else {
         const int d = 2 * (u % (D / 2)), lg = u / (D / 2) & 3, hf = u / (2 * D);     // tokens 32 hf + 16 (x / 4) + 4 lg + x % 4 of two dims
         const i8* f = in + (size_t)((d / 16 * 4 + lg) * 16 + d % 16) * 16 + 8 * hf;
-        uint2_t w[2] = {{0, 0}, {0, 0}};
-        if (there) {
-            w[0] = *gptr((const uint2_t*)f);
-            w[1] = *gptr((const uint2_t*)(f + 16));
-        }
-        char* q = out + (int64_t)(32 * hf + 4 * lg) * row + (size_t)d * es;
+        const uint2_t w0 = *gptr((const uint2_t*)f), w1 = *gptr((const uint2_t*)(f + 16));   // (of block 0 where there is none)
+        const int t0 = 32 * hf + 4 * lg;
+        char* q = out + t0 * row + (size_t)d * es;
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            const int key = 32 * hf + 16 * (x >> 2) + 4 * lg + (x & 3);
-            if (i0 + key >= 0 && i0 + key < a.n) {
-                const float s = p0 + key < end ? sc : 0.f;
-                const float v0 = (float)(i8)(w[0][x >> 2] >> (8 * (x & 3))) * s, v1 = (float)(i8)(w[1][x >> 2] >> (8 * (x & 3))) * s;
-                char* o = q + (16 * (x >> 2) + (x & 3)) * row;
-                if (a.dt == TCQ_F32) *gptr((uint2_t*)o) = uint2_t{__float_as_uint(v0), __float_as_uint(v1)};
-                else *gptr((u32*)o) = kv_pair(v0, v1, a.dt);
-            }
+            const int key = t0 + 16 * (x >> 2) + (x & 3);
+            if (key < lo || key >= hi) continue;
+            const float v0 = key < have ? i8_f32(w0[x >> 2], x & 3) * sc : 0.f, v1 = key < have ? i8_f32(w1[x >> 2], x & 3) * sc : 0.f;
+            char* o = q + (16 * (x >> 2) + (x & 3)) * row;
+            if (a.dt == TCQ_F32) *gptr((uint2_t*)o) = uint2_t{__float_as_uint(v0), __float_as_uint(v1)};
+            else *gptr((u32*)o) = kv_pair(v0, v1, a.dt);
         }
     }
 }
@@ -256,7 +279,8 @@ __device__ __forceinline__ void widen(uint4_t w, half8_t& a, half8_t& b) {
 //                 exponent; a unit that changes rescales them exactly, down to 2^-60 of the largest scale so far); the probabilities' sum
 //                 is their product with ones.
 // The outputs are rescaled only once a maximum is a factor of 256 past the one that they stand on.
-// A wave holds one block's keys or values at a time and leaves the overlap of loads, matrix and vector instructions to the other waves of its
+// A wave holds one block's keys or values at a time (D = 256, where two waves a SIMD are all that fit: the next block's keys too, 131000 keys
+// 27.5 -> 25 us) and leaves the overlap of loads, matrix and vector instructions to the other waves of its
 // SIMD (four of them for D up to 128): one wave issues a vector instruction every 7 to 13 cycles here, four together every 3 to 5. With the next
 // block's keys and values already under way (twice the registers, half the waves) 968 causal rows of 16 x 128 took 19.5 us instead of
 // 16.6, 4096 rows 140 instead of 131, and 131000 keys the same 27.5.
@@ -264,7 +288,7 @@ template <int D, int W, int RT>
 __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_attend(KvAttend a) {
     constexpr int KS = D / 64, DTL = D / 16;
     constexpr int QN = RT * KS;                                      // (tile, K step) pairs of query digits, one a wave
-    static_assert(QN <= W, "");
+    static_assert(QN <= W, "a wave makes the digits of at most one pair");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
     const int split = blockIdx.x % a.S, tile = blockIdx.x / a.S, h = blockIdx.y, b = blockIdx.z;
@@ -315,6 +339,8 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
         wq[0] = gptr((const uint4_t*)at)[0];
         wq[1] = gptr((const uint4_t*)at)[1];
     }
+    constexpr bool AHEAD = D == 256 && W == 4;                       // the next block's keys are fetched while this one's values are used
+    if (AHEAD && j < nb) load_k(j);
     auto local_barrier = [] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
         __builtin_amdgcn_s_barrier();
@@ -384,11 +410,11 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
         for (int dt = 0; dt < DTL; ++dt) O[rt][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     auto block = [&](auto edge) {
-        load_k(j);
-        float c[RT], f[RT][16];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            c[rt] = __builtin_amdgcn_ldexpf(qs[rt] * sk, E[rt]);
+        if (!AHEAD) load_k(j);
+        const float svj = sv;
+        float c, f[16];                                              // one tile's scores at a time
+        auto scores = [&](int rt) {
+            c = __builtin_amdgcn_ldexpf(qs[rt] * sk, E[rt]);
             int4_t hi[4], lo[4];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -400,18 +426,21 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 }
             }
 #pragma unroll
-            for (int x = 0; x < 16; ++x) f[rt][x] = (float)((hi[x >> 2][x & 3] << 8) + lo[x >> 2][x & 3]);
-        }
-        __builtin_amdgcn_sched_barrier(0);                           // (the values' loads no earlier: they take the keys' registers)
-        load_v(j);
+            for (int x = 0; x < 16; ++x) f[x] = (float)((hi[x >> 2][x & 3] << 8) + lo[x >> 2][x & 3]);
+            if (rt == RT - 1) {
+                __builtin_amdgcn_sched_barrier(0);                   // (the values' loads no earlier: they take the keys' registers)
+                load_v(j);
+                if (AHEAD && j + step < nb) load_k(j + step);
+            }
+        };
         auto left = [&](int rt, int x) { return 16 * (x >> 2) + (x & 3) < vend[rt] - j * KB - 4 * lg; };   // key x of this lane group is visible
         auto largest = [&](int rt) {
             if constexpr (edge)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) f[rt][x] = left(rt, x) ? f[rt][x] : -__builtin_inff();
-            float mx = f[rt][0];
+                for (int x = 0; x < 16; ++x) f[x] = left(rt, x) ? f[x] : -__builtin_inff();
+            float mx = f[0];
 #pragma unroll
-            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, f[rt][x]);
+            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, f[x]);
             return mx;
         };
         auto across = [&](float mx) {
@@ -419,12 +448,13 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
             return fmaxf(mx, lane_xor(mx, 32, lane));
         };
         if constexpr (RT == 1) {
+            scores(0);
             const float mx = across(largest(0));
             const bool none = edge && mx == -__builtin_inff();       // the row sees no key of the block
-            const float mb = none ? 0.f : mx * c[0];
+            const float mb = none ? 0.f : mx * c;
             float p[16], lb = 0.f;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[0][x], c[0], -mb));
+            for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[x], c, -mb));
             if constexpr (edge)                                      // also where c is 0 and the product above NaN
 #pragma unroll
                 for (int x = 0; x < 16; ++x) p[x] = left(0, x) ? p[x] : 0.f;
@@ -447,7 +477,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 for (int dt = 0; dt < DTL; ++dt) O[0][dt] *= al;
                 mr[0] = up ? mb : mr[0];
             }
-            const float w = none ? 0.f : __builtin_amdgcn_exp2f(mb - mr[0]), be = none ? 0.f : w * (sv * (1.f / PC));
+            const float w = none ? 0.f : __builtin_amdgcn_exp2f(mb - mr[0]), be = none ? 0.f : w * (svj * (1.f / PC));
             l[0] = __builtin_fmaf(w, lb, l[0]);
 #pragma unroll
             for (int dt = 0; dt < DTL; ++dt) {
@@ -459,24 +489,25 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
         } else {
             // the unit of the outputs, changed when the scale leaves [unit / 64, unit]
             int shift = 0;
-            const int es = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(sv));
+            const int es = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(svj));
             if (es > er || es < er - 6) {                            // uniform
-                top = fmaxf(top, sv);
+                top = fmaxf(top, svj);
                 const int ne = max(min(es, 127), __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) - 60);
                 shift = er - ne;
                 er = ne;
             }
             // p sv = 2^(s - m + lu) rho; their sum in units of the probabilities is iu times what the MFMA adds
-            const float lu = __builtin_amdgcn_logf(sv) - (float)er, iu = __builtin_amdgcn_exp2f(-lu);
+            const float lu = __builtin_amdgcn_logf(svj) - (float)er, iu = __builtin_amdgcn_exp2f(-lu);
             half8_t P[RT][2], ones;
 #pragma unroll
             for (int x = 0; x < 8; ++x) ones[x] = (_Float16)1.f;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
+                scores(rt);
                 float mx = largest(rt);
-                if (shift || __builtin_amdgcn_ballot_w64(mx * c[rt] > mr[rt] + 8.f)) {   // uniform
+                if (shift || __builtin_amdgcn_ballot_w64(mx * c > mr[rt] + 8.f)) {   // uniform
                     mx = across(mx);
-                    const float mb = edge && mx == -__builtin_inff() ? mx : mx * c[rt];
+                    const float mb = edge && mx == -__builtin_inff() ? mx : mx * c;
                     const bool up = mb > mr[rt] + 8.f;
                     const float al = up ? __builtin_amdgcn_exp2f(mr[rt] - mb) : 1.f, ak = __builtin_amdgcn_ldexpf(al, shift);
                     l[rt] *= al;
@@ -487,7 +518,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 const float mz = edge && mr[rt] == -__builtin_inff() ? 0.f : mr[rt] - lu;
                 float p[16];
 #pragma unroll
-                for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[rt][x], c[rt], -mz));
+                for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[x], c, -mz));
                 if constexpr (edge)
 #pragma unroll
                     for (int x = 0; x < 16; ++x) p[x] = left(rt, x) ? p[x] : 0.f;
@@ -512,63 +543,58 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     const int whole = all / KB;                                      // blocks that every row sees whole (rows past the last one do not count)
     while (j < min(nb, whole)) block(std::false_type());
     while (j < nb) block(std::true_type());
-    // merge the waves through LDS: statistics and outputs, wave w summing its share of the dim tiles
-    __syncthreads();
-    constexpr int NT = RT * DTL, WD = NT < W ? NT : W, DW = NT / WD; // dim tiles, waves that sum, dim tiles of each
+    // merge the waves through LDS, a row tile at a time: statistics and outputs, wave w summing its share of the dim tiles
+    constexpr int WD = DTL < W ? DTL : W, DW = DTL / WD;             // waves that sum, dim tiles of each
     float4_t* x = (float4_t*)lds;
-    float *sm = (float*)(lds + W * NT * 1024), *sl = sm + 16 * RT * W;
+    float *sm = (float*)(lds + W * DTL * 1024), *sl = sm + 16 * W;
     const float rho = RT == 1 ? 1.f : __builtin_amdgcn_ldexpf(1.f, er);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+        __syncthreads();
         float s = l[rt];
         if (RT == 1) {
             s += lane_xor(s, 16, lane);
             s += lane_xor(s, 32, lane);
         }
         if (lg == 0) {
-            sm[16 * (RT * wave + rt) + lr] = mr[rt];
-            sl[16 * (RT * wave + rt) + lr] = s;
+            sm[16 * wave + lr] = mr[rt];
+            sl[16 * wave + lr] = s;
         }
 #pragma unroll
-        for (int dt = 0; dt < DTL; ++dt) x[(wave * NT + rt * DTL + dt) * 64 + lane] = RT == 1 ? O[rt][dt] : O[rt][dt] * rho;
-    }
-    __syncthreads();
-    if (wave >= WD) return;
-    constexpr int TW = DW < DTL ? 1 : DW / DTL, TD = DW / TW;        // row tiles that a wave sums, dim tiles of each
-#pragma unroll
-    for (int i = 0; i < TW; ++i) {
-        const int rt = TW > 1 ? wave * TW + i : wave * DW / DTL, d0 = TW > 1 ? 0 : wave * DW % DTL, r = row0 + 16 * rt + lr;
-        if (r >= nrows) continue;
+        for (int dt = 0; dt < DTL; ++dt) x[(wave * DTL + dt) * 64 + lane] = RT == 1 ? O[rt][dt] : O[rt][dt] * rho;
+        __syncthreads();
+        const int r = row0 + 16 * rt + lr;
+        if (wave >= WD || r >= nrows) continue;
         float mx = -__builtin_inff(), lsum = 0.f, wt[W];
 #pragma unroll
-        for (int w = 0; w < W; ++w) mx = fmaxf(mx, sm[16 * (RT * w + rt) + lr]);
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, sm[16 * w + lr]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             // a wave without a visible key has l = 0 and weight 0; one whose scores are NaN has l = NaN and weight NaN
-            const float mw = sm[16 * (RT * w + rt) + lr], lw = sl[16 * (RT * w + rt) + lr];
+            const float mw = sm[16 * w + lr], lw = sl[16 * w + lr];
             wt[w] = mw == -__builtin_inff() ? lw : __builtin_amdgcn_exp2f(mw - mx);
             lsum = __builtin_fmaf(wt[w], lw, lsum);
         }
         int hq;
         const int t = token(r, hq);
         const size_t row = (size_t)(c0 + t) * (a.Hk * a.G) + hq;
-        if (a.S > 1 && d0 == 0 && lg == 0) {
+        if (a.S > 1 && wave == 0 && lg == 0) {
             a.stat[(row * a.S + split) * 2] = mx;
             a.stat[(row * a.S + split) * 2 + 1] = lsum;
         }
         const float inv = lsum == 0.f ? 0.f : 1.f / lsum;            // a row that sees no key: zeros
 #pragma unroll
-        for (int k = 0; k < TD; ++k) {
-            const int dt = d0 + k;
-            float4_t s = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < DW; ++k) {
+            const int dt = wave * DW + k;
+            float4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float4_t y = x[(w * NT + rt * DTL + dt) * 64 + lane];
+                const float4_t y = x[(w * DTL + dt) * 64 + lane];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(wt[w], y[e], s[e]);
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(wt[w], y[e], v[e]);
             }
-            if (a.S > 1) *gptr((float4_t*)(a.part + (row * a.S + split) * D + 16 * dt + 4 * lg)) = s;
-            else store4(a.o + row * D + 16 * dt + 4 * lg, s * inv, a.bf16);
+            if (a.S > 1) *gptr((float4_t*)(a.part + (row * a.S + split) * D + 16 * dt + 4 * lg)) = v;
+            else store4(a.o + row * D + 16 * dt + 4 * lg, v * inv, a.bf16);
         }
     }
 }
@@ -604,10 +630,11 @@ __global__ __launch_bounds__(KT) void k_kv8_join_few(KvAttend a) {
 }
 
 // More splits: grid (most x Hq, 1, B), one row a workgroup. The first wave works out the weights (lane = split) while thread (g, 4 dims) has
-// its first eight of every (KT / (D / 4))th split under way.
+// its first eight of every (JT / (D / 4))th split under way.
+constexpr int JT = 1024;         // its threads
 template <int D>
-__global__ __launch_bounds__(KT) void k_kv8_join(KvAttend a) {
-    constexpr int TD = D / 4, NG = KT / TD, SR = MAX_SPLITS / 64, U = 8;
+__global__ __launch_bounds__(JT) void k_kv8_join(KvAttend a) {
+    constexpr int TD = D / 4, NG = JT / TD, SR = MAX_SPLITS / 64, U = 8;
     __shared__ float4_t sums[NG][TD];
     __shared__ float wt[MAX_SPLITS], tot;
     const int tid = threadIdx.x, d = tid % TD, g = tid / TD, S = a.S, b = blockIdx.z, Hq = a.Hk * a.G, t = blockIdx.x / Hq;
@@ -664,8 +691,8 @@ __global__ __launch_bounds__(KT) void k_kv8_join(KvAttend a) {
     store4(a.o + row * D + 4 * d, acc * (tot == 0.f ? 0.f : 1.f / tot), a.bf16);
 }
 
-size_t kv_attend_lds(int D, int W, int RT) {     // the waves' outputs and statistics, or the query digits and maxima before them
-    return max((size_t)W * RT * ((D / 16) * 1024 + 128), (size_t)RT * (D / 64) * (2048 + 64));
+size_t kv_attend_lds(int D, int W, int RT) {     // the waves' outputs and statistics of a row tile, or the query digits and maxima before them
+    return max((size_t)W * ((D / 16) * 1024 + 128), (size_t)RT * (D / 64) * (2048 + 64));
 }
 bool kv_dim(int D) { return D == 64 || D == 128 || D == 256; }
 bool kv_size(int B, int H, int nblk) { return B > 65535 || H > 65535 || nblk > (1 << 25) - 1; }
@@ -710,7 +737,7 @@ extern "C" int tcq_kv8_append(const void* k, int64_t k_tok, int64_t k_head, cons
     if (((uintptr_t)k | (uintptr_t)v) % 2 || ((uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)tail) % 16 || (uintptr_t)scale % 8) return TCQ_ERR_ALIGN;
     const bool vec = !(((uintptr_t)k | (uintptr_t)v) % 16) && !((k_tok | k_head | v_tok | v_head) % 8);
     const KvAppend a = {(const u16*)k, (const u16*)v, k_tok, k_head, v_tok, v_head, cu, start, (i8*)k8, (i8*)v8, scale, (u16*)tail,
-                        rows, most, H, D, nblk};
+                        rows, most, H, D, nblk, max(k_tok, v_tok) < (1 << 24) && min(k_tok, v_tok) >= 0};
     const dim3 grid((u32)(2 * min((int64_t)nblk, ((int64_t)most + KB - 2) / KB + 1)), H, B);
     hipStream_t st = (hipStream_t)stream;
 #define KV_APPEND(N)                                                                                    \
@@ -776,7 +803,7 @@ extern "C" int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int 
             const int e = launch_status();                                                                              \
             if (e) return e;                                                                                            \
             constexpr int PR = KT / (N / 4);                                                                            \
-            if (S > 8) launch_k(k_kv8_join<N>, dim3((u32)most * Hq, 1, B), dim3(KT), 0, st, a);                         \
+            if (S > 8) launch_k(k_kv8_join<N>, dim3((u32)most * Hq, 1, B), dim3(JT), 0, st, a);                         \
             else launch_k(k_kv8_join_few<N>, dim3(((u32)most * Hq + PR - 1) / PR, 1, B), dim3(KT), 0, st, a);             \
         }                                                                                                               \
     } while (0)

@@ -493,7 +493,8 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
     """Attention of q (rows, Hq, D; BF16 / FP16, any token and head strides) over the first lens[b] rows (int32, on the device) of every
     sequence of the cache, Hq a multiple of its heads: o (rows, Hq, D). B equal shares of the rows, or cu and most as in kv8_append. With
     causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended). scale: of the scores,
-    1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work alone."""
+    1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work alone. A row that sees
+    nothing is zeros; rows of no sequence (and a sequence's past `most`) are left as they were in o, and hold anything in a new one."""
     B, H, n, E = _kv8(cache, 'kv8_attend')
     size, sq, dt = q.shape, q.stride(), q.dtype
     if not (len(size) == 3 and size[2] == 16 * E and sq[2] == 1 and size[1] > 0 and size[1] % H == 0):
@@ -513,7 +514,7 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
         L = _lib.lib()
         floats = L.tcq_kv8_attend_floats(rows, most, B, Hq, H, D, keys)
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        rc = L.tcq_kv8_attend(pq, sq[0], sq[1], DTYPE[dt], pc, pl, rows, most, B, Hq, H, D, n, pk8, pv8, ps, causal,
+        rc = L.tcq_kv8_attend(pq, sq[0] if rows > 1 else 0, sq[1] if Hq > 1 else 0, DTYPE[dt], pc, pl, rows, most, B, Hq, H, D, n, pk8, pv8, ps, causal,
                               D ** -0.5 if scale is None else scale, keys, part.data_ptr() if floats else None, po, stream())
         if rc:
             _lib.failed('tcq_kv8_attend', rc)
