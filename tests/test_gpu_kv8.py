@@ -402,3 +402,72 @@ def test_decode_loop_as_one_graph():
         n = [P + i + 1] * B
         kk, vv = K.kv8_read(caches[1], ints([0, 0]), ints(n), n[0], FP)
         close(o, reference(q, kk, vv, n, [1, 1], 2, True))
+
+
+FORMS = [([90, 400], 8, 1, 256, 2, 500), ([5000, 3000], 16, 8, 128, 1, 5000), ([5000, 100], 4, 1, 64, 3, 5000), ([9000], 8, 1, 256, 1, 9000),
+         ([600, 900], 16, 8, 128, 520, 900), ([300, 200], 8, 2, 64, 70, 300)]
+
+
+@pytest.mark.parametrize('lens,Hq,Hk,D,M,keys', FORMS)
+def test_attend_replays_with_other_lengths(lens, Hq, Hk, D, M, keys):
+    """One workgroup a tile, keys in few and in many parts, many rows: captured once, replayed with lengths and queries that change, eager
+    calls in between; every replay is the eager call's result."""
+    from yanlongvla_amd import kernels as K
+    cache, _, _ = fill(lens, Hk, D, seed=51)
+    B = len(lens)
+    q, n = rand(B * M, Hq, D, seed=52), ints(lens)
+    K.kv8_attend(q, cache, n, keys=keys)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        o = K.kv8_attend(q, cache, n, keys=keys)
+    for i, cut in enumerate((0, 70, 1, 10 ** 6, 0)):
+        q.copy_(rand(B * M, Hq, D, seed=60 + i))
+        n.copy_(ints([max(0, x - cut) for x in lens]))
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, K.kv8_attend(q, cache, n, keys=keys))
+        assert cut < 10 ** 6 or (o == 0).all()
+
+
+def test_calls_on_two_streams_at_once():
+    """Attention in parts of two caches on two streams, a third cache appended to beside them, the results those of one after the other."""
+    from yanlongvla_amd import kernels as K
+    jobs = []
+    for i, (lens, Hq, Hk, D, M, keys) in enumerate(FORMS[1:4]):
+        cache, _, _ = fill(lens, Hk, D, seed=70 + i)
+        q = rand(len(lens) * M, Hq, D, seed=80 + i)
+        jobs.append((cache, q, ints(lens), keys, K.kv8_attend(q, cache, ints(lens), keys=keys)))
+    one, two = (K.kv8_cache(1, 8, 128, 3000, DEV) for _ in range(2))
+    k, v = rand(3000, 8, 128, seed=90), rand(3000, 8, 128, seed=91)
+    K.kv8_append(one, k, v, ints([0]))
+    starts = [ints([a]) for a in range(0, 3000, 100)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [[] for _ in jobs]
+    for _ in range(10):
+        for (cache, q, n, keys, _), st, g in zip(jobs, streams, got):
+            with torch.cuda.stream(st):
+                g.append(K.kv8_attend(q, cache, n, keys=keys))
+        for a in starts[:3]:
+            K.kv8_append(two, k[:100], v[:100], a)
+    for i, a in enumerate(starts):
+        K.kv8_append(two, k[100 * i:100 * i + 100], v[100 * i:100 * i + 100], a)
+    torch.cuda.synchronize()
+    for job, g in zip(jobs, got):
+        assert all(torch.equal(x, job[4]) for x in g)
+    assert all(torch.equal(x, y) for x, y in zip(one[:3], two[:3]))
+
+
+def test_more_row_tiles_than_a_grid_axis_holds():
+    """65600 rows of 16 heads on one KV head: 65600 tiles of 16 rows; the first, the last and those in between, causal and not."""
+    from yanlongvla_amd import kernels as K
+    rows, D, n = 65600, 64, 150
+    cache, _, _ = fill([n], 1, D, seed=95)
+    k, v = K.kv8_read(cache, ints([0]), ints([n]), n, FP)
+    q = rand(rows, 16, D, seed=96)
+    o = K.kv8_attend(q, cache, ints([n]), causal=False)
+    for at in (0, 60, 90, 32000, 65500):
+        close(o[at:at + 100], reference(q[at:at + 100], k, v, [n], [100], 16, False))
+    o = K.kv8_attend(q, cache, ints([n]), torch.full_like(q, 9.0))
+    assert (o[:rows - n] == 0).all()
+    close(o[rows - n:], reference(q[rows - n:], k, v, [n], [n], 16, True))

@@ -226,6 +226,7 @@ struct KvAttend {
     u16* o;                                  // (rows, Hq, D)
     float sl;                                // score scale * log2 e
     int rows, most, G, Hk, nblk, causal, bf16, S;
+    int last;                                // the row tile of blockIdx.z = 0
 };
 
 constexpr float QC = 32512.f;    // query digits: 127 * 256, the largest value whose rounded high digit stays within 127
@@ -279,11 +280,15 @@ __device__ __forceinline__ void widen(uint4_t w, half8_t& a, half8_t& b) {
 //                 exponent; a unit that changes rescales them exactly, down to 2^-60 of the largest scale so far); the probabilities' sum
 //                 is their product with ones.
 // The outputs are rescaled only once a maximum is a factor of 256 past the one that they stand on.
-// A wave holds one block's keys or values at a time (D = 256, where two waves a SIMD are all that fit: the next block's keys too, 131000 keys
-// 27.5 -> 25 us) and leaves the overlap of loads, matrix and vector instructions to the other waves of its
-// SIMD (four of them for D up to 128): one wave issues a vector instruction every 7 to 13 cycles here, four together every 3 to 5. With the next
-// block's keys and values already under way (twice the registers, half the waves) 968 causal rows of 16 x 128 took 19.5 us instead of
-// 16.6, 4096 rows 140 instead of 131, and 131000 keys the same 27.5.
+// A wave holds one block's keys or values at a time and leaves the overlap of loads, matrix and vector instructions to the other waves of
+// its SIMD (four of them for D up to 128): one wave issues a vector instruction every 7 to 13 cycles here, four together every 3 to 5. With
+// the next block's keys and values already under way (twice the registers, half the waves) 968 causal rows of 16 x 128 took 19.5 us instead
+// of 16.6, 4096 rows 140 instead of 131. D = 256 in four waves, where two a SIMD are all that fit, does fetch the next keys: 131000 keys of
+// two sequences 25.5 us instead of 27.5 (4.6 TB/s; 16 sequences of 8 heads x 128 behind 8192 keys 40.8 us, 5.0 TB/s).
+// Grid (Hk x parts, B, row tiles): workgroups go to the eight XCDs in turn, so with eight KV heads an XCD's L2 sees one head's keys, and a
+// tile's workgroups of all sequences come before the next tile's, the last tiles first, as they see the most keys. With the tiles of a head
+// side by side and the first ones first: 968 causal rows of 16 x 128 16.7 us against 13.2, of 8 x 256 16.8 against 14.6, 4096 rows 129
+// against 113, 90 rows behind 1936 keys, 8 sequences of 16 x 64 23.4 against 17 (2 x 1024 rows behind 4096 keys 103 against 104).
 template <int D, int W, int RT>
 __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_attend(KvAttend a) {
     constexpr int KS = D / 64, DTL = D / 16;
@@ -291,7 +296,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     static_assert(QN <= W, "a wave makes the digits of at most one pair");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
-    const int split = blockIdx.x % a.S, tile = blockIdx.x / a.S, h = blockIdx.y, b = blockIdx.z;
+    const int split = blockIdx.x % a.S, h = blockIdx.x / a.S, b = blockIdx.y, tile = a.last - blockIdx.z;
     const int c0 = a.cu ? max(0, a.cu[b]) : b * a.most, count = a.cu ? a.cu[b + 1] - c0 : a.most;
     const int m = min(min(count, a.most), a.rows - c0);              // rows computed here
     const int L = min(max(a.lens[b], 0), a.nblk * KB);
@@ -691,6 +696,7 @@ __global__ __launch_bounds__(JT) void k_kv8_join(KvAttend a) {
     store4(a.o + row * D + 4 * d, acc * (tot == 0.f ? 0.f : 1.f / tot), a.bf16);
 }
 
+constexpr int64_t MAX_Z = 65535;  // the grid's z
 size_t kv_attend_lds(int D, int W, int RT) {     // the waves' outputs and statistics of a row tile, or the query digits and maxima before them
     return max((size_t)W * ((D / 16) * 1024 + 128), (size_t)RT * (D / 64) * (2048 + 64));
 }
@@ -785,20 +791,23 @@ extern "C" int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int 
     const KvPlan plan = kv_plan(B, most, G, Hk, D, keys);
     const int S = plan.S;
     const int64_t tiles = ((int64_t)most * G + 16 * plan.RT - 1) / (16 * plan.RT);
-    if (tiles * S > 0x7fffffff || (int64_t)most * Hq > 0x7fffffff || (int64_t)rows * Hq > 0x7fffffff) return TCQ_ERR_UNSUPPORTED;
+    if ((int64_t)most * Hq > 0x7fffffff || (int64_t)rows * Hq > 0x7fffffff) return TCQ_ERR_UNSUPPORTED;
     if (S > 1 && !part) return TCQ_ERR_ARG;
     if (((uintptr_t)q | (uintptr_t)k8 | (uintptr_t)v8 | (uintptr_t)o | (uintptr_t)part) % 16 || (q_tok | q_head) % 8 || (uintptr_t)scale % 8)
         return TCQ_ERR_ALIGN;
     KvAttend a = {(const u16*)q, q_tok, q_head, cu, lens, (const i8*)k8, (const i8*)v8, scale, part, part + (S > 1 ? (size_t)rows * Hq * S * D : 0),
-                  (u16*)o, score_scale * 1.44269504088896341f, rows, most, G, Hk, nblk, causal != 0, dtype == TCQ_BF16, S};
+                  (u16*)o, score_scale * 1.44269504088896341f, rows, most, G, Hk, nblk, causal != 0, dtype == TCQ_BF16, S, 0};
     hipStream_t st = (hipStream_t)stream;
 #define KV_ATTEND(N)                                                                                                    \
     do {                                                                                                                \
-        const dim3 grid((u32)(tiles * S), Hk, B);                                                                       \
         const size_t lds = kv_attend_lds(N, plan.W, plan.RT);                                                           \
-        if (plan.W == 8) launch_k(k_kv8_attend<N, 8, 1>, grid, dim3(512), lds, st, a);                                  \
-        else if (N != 128 || plan.RT == 1) launch_k(k_kv8_attend<N, 4, 1>, grid, dim3(256), lds, st, a);                \
-        else launch_k(k_kv8_attend<128, 4, 2>, grid, dim3(256), lds, st, a);                                            \
+        for (int64_t left = tiles; left > 0; left -= MAX_Z) {                                                           \
+            const dim3 grid((u32)(Hk * S), B, (u32)min(left, MAX_Z));                                                   \
+            a.last = (int)(left - 1);                                                                                   \
+            if (plan.W == 8) launch_k(k_kv8_attend<N, 8, 1>, grid, dim3(512), lds, st, a);                              \
+            else if (N != 128 || plan.RT == 1) launch_k(k_kv8_attend<N, 4, 1>, grid, dim3(256), lds, st, a);            \
+            else launch_k(k_kv8_attend<128, 4, 2>, grid, dim3(256), lds, st, a);                                        \
+        }                                                                                                               \
         if (S > 1) {                                                                                                    \
             const int e = launch_status();                                                                              \
             if (e) return e;                                                                                            \
