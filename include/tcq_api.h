@@ -336,13 +336,14 @@ int tcq_kv8_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, 
 int tcq_kv8_read(const int8_t* k8, const int8_t* v8, const float* scale, const int32_t* first, const int32_t* lens, int n, int B, int H, int D,
                  int nblk, void* k, void* v, int dtype, tcq_stream_t stream);
 /* Attention over the cache: o = softmax(score_scale q k^T) v, query head i over KV head i / (Hq / Hk), sequence b's rows cu[b] ..
- * cu[b + 1] - 1 (cu NULL: most rows each) of q (rows, Hq, D; BF16 or F16, strides in elements) over its first lens[b] positions; with
- * causal, row i of n sees positions j <= lens[b] - n + i. o (rows, Hq, D) contiguous, of q's type. A row that sees nothing is zeros; a query
- * row with a value that is not finite is NaN; rows of no sequence are left as they were. keys: about the most positions that a
- * sequence has (it sets how far the work is split, never the result's meaning). part: workspace of tcq_kv8_attend_floats(...) floats,
- * 16-byte aligned (NULL where that is 0), not shared by calls that overlap. Scores from the query as 16-bit integers (within 2^-16 of the
- * row's largest value) and the probabilities as 16-bit integers of their block's maximum, exact int32 products with the codes, FP32
- * maximum, sum and outputs (many rows of D = 128: FP16 probabilities of the running maximum instead). */
+ * cu[b + 1] - 1 (cu NULL: most rows each) of q (rows, Hq, D; BF16 or F16, 16-byte aligned, strides in elements, multiples of 8) over its
+ * first lens[b] positions; with causal, row i of n sees positions j <= lens[b] - n + i. o (rows, Hq, D) contiguous, of q's type. A row
+ * that sees nothing is zeros; another query row with a value that is not finite is NaN; rows of no sequence are left as they were. keys:
+ * about the most positions that a sequence has (it sets how far the work is split, never the result's meaning). part: workspace of
+ * tcq_kv8_attend_floats(...) floats, 16-byte aligned (NULL where that is 0), not shared by calls that overlap. Scores from the query as
+ * 16-bit integers (within 2^-16 of the row's largest value) and the probabilities as 16-bit integers of their block's maximum, exact
+ * int32 products with the codes, FP32 maximum, sum and outputs (many rows of D up to 128: FP16 probabilities of the running maximum
+ * instead). */
 int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, const int32_t* lens, int rows, int most, int B,
                    int Hq, int Hk, int D, int nblk, const int8_t* k8, const int8_t* v8, const float* scale, int causal, float score_scale,
                    int keys, float* part, void* o, tcq_stream_t stream);

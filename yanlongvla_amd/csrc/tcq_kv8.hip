@@ -159,7 +159,7 @@ __device__ __forceinline__ u32 kv_pair(float x, float y, int dt) {   // (finite 
 }
 
 // grid (2 x D / 64 x blocks a window may touch, H, B): 256 pieces of 16 values of a block's keys (even block index) or values; k, v (B, n, H, D),
-// row i of sequence b is position first[b] + i, zeros from lens[b] on. MI355X: 6 x 1024 rows, 8 heads of 128 11.7 us (38 MB, 3.2 TB/s).
+// row i of sequence b is position first[b] + i, zeros from lens[b] on. MI355X: 6 x 1024 rows, 8 heads of 128 11.6 us (38 MB, 3.2 TB/s).
 template <int D>
 __global__ __launch_bounds__(KT) void k_kv8_read(KvRead a) {
     const int b = blockIdx.z, h = blockIdx.y, bx = blockIdx.x / (D / 64), val = bx & 1, u = blockIdx.x % (D / 64) * KT + threadIdx.x;
@@ -605,6 +605,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
 }
 
 // The splits' outputs of a row joined, weights exp2(m_s - max m). Few splits (at most 8): D / 4 threads a row, 4 dims each, every load at entry.
+// A launch and two memory latencies: 256 rows x 8 parts x 128 4.5 us.
 template <int D>
 __global__ __launch_bounds__(KT) void k_kv8_join_few(KvAttend a) {
     constexpr int TD = D / 4, MS = 8;
@@ -635,7 +636,7 @@ __global__ __launch_bounds__(KT) void k_kv8_join_few(KvAttend a) {
 }
 
 // More splits: grid (most x Hq, 1, B), one row a workgroup. The first wave works out the weights (lane = split) while thread (g, 4 dims) has
-// its first eight of every (JT / (D / 4))th split under way.
+// its first eight of every (JT / (D / 4))th split under way. 16 rows x 128 parts x 256 4.0 us (with 256 threads 4.8).
 constexpr int JT = 1024;         // its threads
 template <int D>
 __global__ __launch_bounds__(JT) void k_kv8_join(KvAttend a) {
@@ -704,19 +705,21 @@ bool kv_dim(int D) { return D == 64 || D == 128 || D == 256; }
 bool kv_size(int B, int H, int nblk) { return B > 65535 || H > 65535 || nblk > (1 << 25) - 1; }
 
 // How a call is split: the waves W of a workgroup, which take the blocks of 16 RT rows of a KV head in turn, and the parts S of their keys.
-//   Two tiles of 16 rows a wave (D = 128) where that still makes two workgroups a CU: 1024 rows behind 4096 keys, 2 sequences of 16 x 8 heads
-//   99 us against 111, 300 rows behind 1000 16.5 against 13.7. (D = 64: 42 us against 36 at 4 x 1024 rows. D = 256: its registers.)
-//   Few rows over up to 16 blocks: one launch of eight waves (968 keys of one sequence, D = 256: 10.5 us against 8.8 in parts of four waves
-//   with their join, but a call from Python 12 us against 16).
-//   Else four waves (968 causal rows of 8 heads x 256 16 us, with eight 20), in as many parts as give every CU a workgroup. Where that is
+//   Two tiles of 16 rows a wave (D up to 128; 256 has no registers left for it) where that still makes two workgroups a CU: 2 x 1024 rows of
+//   16 heads x 128 behind 4096 keys 104 us against 115, 4096 rows 112 against 125, 4 x 1024 rows of 16 heads x 64 28 against 32; with half
+//   as many workgroups it loses (968 rows of 16 x 128 14.5 against 13.2), three or four tiles gain nothing (D = 64: 31).
+//   Few rows over up to 16 blocks: one launch of eight waves (50 rows of 4 sequences behind 800 keys, D = 256: 10.8 us against 12.8 in parts
+//   of four waves with their join, 10 rows of 16 sequences 10.6 against 13.8; one row behind 968 10.0 against 9.0, but a call from Python
+//   12 against 16).
+//   Else four waves (968 causal rows of 8 heads x 256 14.5 us, with eight 18.4), in as many parts as give every CU a workgroup. Where that is
 //   fewer than 4 and the parts stay long, as many as fit: the lengths of a batch differ (16 sequences of 4 to 8 thousand keys, 8 heads of
-//   128: 47 us against 54; of 1.5 to 3 thousand, 64 dims, 22 against 19).
+//   128: 47 us against 58).
 struct KvPlan {
     int W, S, RT;
 };
 KvPlan kv_plan(int B, int most, int G, int Hk, int D, int keys) {
     const int64_t n = (int64_t)most * G, heads = (int64_t)B * Hk, nb = ((int64_t)keys + KB - 1) / KB;
-    if (D == 128 && heads * ((n + 31) / 32) >= 512) return {4, 1, 2};
+    if (D <= 128 && heads * ((n + 31) / 32) >= 512) return {4, 1, 2};
     const int64_t groups = heads * ((n + 15) / 16);
     if (groups <= 256 && nb <= 16) return {8, 1, 1};
     int64_t S = max((int64_t)1, min(256 / groups, (nb + 3) / 4));
@@ -805,8 +808,8 @@ extern "C" int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int 
             const dim3 grid((u32)(Hk * S), B, (u32)min(left, MAX_Z));                                                   \
             a.last = (int)(left - 1);                                                                                   \
             if (plan.W == 8) launch_k(k_kv8_attend<N, 8, 1>, grid, dim3(512), lds, st, a);                              \
-            else if (N != 128 || plan.RT == 1) launch_k(k_kv8_attend<N, 4, 1>, grid, dim3(256), lds, st, a);            \
-            else launch_k(k_kv8_attend<128, 4, 2>, grid, dim3(256), lds, st, a);                                        \
+            else if (N == 256 || plan.RT == 1) launch_k(k_kv8_attend<N, 4, 1>, grid, dim3(256), lds, st, a);            \
+            else launch_k(k_kv8_attend<N == 64 ? 64 : 128, 4, 2>, grid, dim3(256), lds, st, a);                             \
         }                                                                                                               \
         if (S > 1) {                                                                                                    \
             const int e = launch_status();                                                                              \

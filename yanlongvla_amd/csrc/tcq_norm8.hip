@@ -4,6 +4,8 @@
 // The codes do not need the norm: n / scale = 127 m / max|m| with m = h (offset + w), so the sum of squares and max|m| are
 // reduced together, one barrier a row, and the norm only enters the scale. The row stays in registers between the reduction
 // and the codes. Statistics in FP32. Memory bound from a few hundred rows on (7 bytes a value in 16-bit types), else latency.
+// MI355X, BF16: 4000 rows of 4096 22.9 us (115 MB, 5.0 TB/s: the rate of a large copy), one row of 2048 2.7 us (a launch, two memory
+// latencies and one barrier).
 #include "tcq_device.h"
 #include "tcq_launch.h"
 

@@ -3,7 +3,9 @@
 // The angle is taken in turns in FP64 (pos * freq / 2 pi, minus its nearest whole number) and only then rounded to FP32: at
 // position 100000 an FP32 product is off by 4e-3 rad, this one by 1e-11 before the FP32 rounding of a number below one half. A
 // workgroup computes the cosines and sines of its tokens once, into LDS, while the loads of its rows are in flight; every
-// head of the token then uses them.
+// head of the token then uses them. MI355X: 4761 tokens of 32 heads x 64, FP32, 13.8 us (78 MB, 5.7 TB/s, some of it out of the
+// last-level cache: memory bound), 2048 tokens of 24 heads x 128, BF16, 7.7 us (25 MB, 3.3 TB/s: launch, the FP64 angles and one wave of
+// loads per workgroup), one token of the same 2.7 us.
 #include "tcq_device.h"
 #include "tcq_launch.h"
 

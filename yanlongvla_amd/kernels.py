@@ -490,11 +490,12 @@ def kv8_read(cache, first, lens, n, dtype=None):
 
 
 def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=None, keys=None):
-    """Attention of q (rows, Hq, D; BF16 / FP16, any token and head strides) over the first lens[b] rows (int32, on the device) of every
-    sequence of the cache, Hq a multiple of its heads: o (rows, Hq, D). B equal shares of the rows, or cu and most as in kv8_append. With
-    causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended). scale: of the scores,
-    1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work alone. A row that sees
-    nothing is zeros; rows of no sequence (and a sequence's past `most`) are left as they were in o, and hold anything in a new one."""
+    """Attention of q (rows, Hq, D; BF16 / FP16, 16-byte aligned, token and head strides multiples of 8) over the first lens[b] rows (int32,
+    on the device) of every sequence of the cache, Hq a multiple of its heads: o (rows, Hq, D). B equal shares of the rows, or cu and most
+    as in kv8_append. With causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended).
+    scale: of the scores, 1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work
+    alone. A row that sees nothing is zeros; rows of no sequence (and a sequence's past `most`) are left as they were in o, and hold
+    anything in a new one."""
     B, H, n, E = _kv8(cache, 'kv8_attend')
     size, sq, dt = q.shape, q.stride(), q.dtype
     if not (len(size) == 3 and size[2] == 16 * E and sq[2] == 1 and size[1] > 0 and size[1] % H == 0):
