@@ -324,9 +324,10 @@ int tcq_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int
 
 /* Rows into the cache: sequence b's rows cu[b] .. cu[b + 1] - 1 (cu NULL: most rows each) of k, v (rows, H, D), BF16 or F16, token and
  * head strides in elements, go to positions start[b], start[b] + 1, ... What a sequence held from start[b] on is gone; the rows
- * before it in start[b]'s block come from the tail, so start[b] lies at most one whole block before the newest block written
- * (an append that ended at start[b], or one that is taken back by up to 64 rows). Every touched block is quantized anew from its 16-bit
- * rows, so a block's codes depend on its rows alone. Rows past the capacity, past `most` of a sequence or past `rows` are dropped, a
+ * before it in start[b]'s block come from the tail. So start[b] lies at most 64 rows before the furthest position written so far, also
+ * where rows were taken back before (after appends to 200 and, from 140, to 141 it may be 136, not 80: block 1's 16-bit rows are
+ * gone); or it is any multiple of 64 (0: a new sequence), before which no later start goes, and the furthest position counts from there.
+ * Every touched block is quantized anew from its 16-bit rows, so a block's codes depend on its rows alone. Rows past the capacity, past `most` of a sequence or past `rows` are dropped, a
  * negative start counts as 0; a sequence without new rows is left as it is. */
 int tcq_kv8_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int dtype, const int32_t* cu,
                    const int32_t* start, int rows, int most, int B, int H, int D, int nblk, int8_t* k8, int8_t* v8, float* scale, void* tail,

@@ -115,6 +115,37 @@ def test_rows_taken_back(P, M):
     assert all(torch.equal(x, y) for x, y in zip(a[:3], b[:3]))
 
 
+@pytest.mark.parametrize('seed', range(6))
+def test_appends_and_rows_taken_back_at_random(seed):
+    """Starts as the documentation allows them, from the furthest position so far and new beginnings at multiples of 64: the cache is that
+    of the surviving rows."""
+    import random
+    from yanlongvla_amd import kernels as K
+    H, D, room, r = 2, 64, 1200, random.Random(seed)
+    cache, one = (K.kv8_cache(1, H, D, room, DEV) for _ in range(2))
+    k, v = (torch.zeros(room, H, D, dtype=BF, device=DEV) for _ in range(2))
+    least = end = far = 0
+    for i in range(60):
+        low = max(least, far - T)
+        if r.random() < 0.1 and end >= T:
+            start = r.randrange(0, end // T + 1) * T
+            if start < low:
+                least = far = start
+        else:
+            start = end if r.random() < 0.4 else r.randint(min(low, end), end)
+        n = r.choice((1, 1, 2, 7, 33, 64, 65, 130, 200))
+        n = min(n, room - start)
+        if n == 0:
+            break
+        k[start:start + n], v[start:start + n] = rand(n, H, D, seed=1000 * seed + 2 * i), rand(n, H, D, seed=1000 * seed + 2 * i + 1)
+        K.kv8_append(cache, k[start:start + n], v[start:start + n], ints([start]))
+        end = start + n
+        far = max(far, end)
+    K.kv8_append(one, k[:end], v[:end], ints([0]))
+    got, want = ([x[0] for x in K.kv8_read(c, ints([0]), ints([end]), end, FP)] for c in (cache, one))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_views_other_sequences_and_the_capacity():
     """Rows as unaligned views of a wider row; a sequence without new rows and the blocks before the new ones stay; rows past the
     capacity, past `most` and past the tensor are dropped."""

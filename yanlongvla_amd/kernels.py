@@ -452,8 +452,9 @@ def _most(what, rows, B, cu, most):
 def kv8_append(cache, k, v, start, cu=None, most=None):
     """Writes rows k, v (rows, H, D; the type of cache.tail, any token and head strides) into the cache from position start[b] (B, int32, on
     the device) of every sequence on: B equal shares of the rows, or rows cu[b] .. cu[b + 1] - 1 (cu (B + 1,) int32 on the device, most: at
-    least the rows of any sequence). What was held from start[b] on is replaced; start[b] may lie up to 64 rows before the last
-    append's end. Rows past the capacity are dropped (see tcq_kv8_append)."""
+    least the rows of any sequence). What was held from start[b] on is replaced; start[b] lies at most 64 rows before
+    the furthest position written so far (also where rows were taken back before), or is a multiple of 64, a new beginning before which no
+    later start goes. Rows past the capacity are dropped (see tcq_kv8_append)."""
     B, H, n, E = _kv8(cache, 'kv8_append')
     size, sk, sv, dt = k.shape, k.stride(), v.stride(), k.dtype
     if not (len(size) == 3 and size == v.shape and size[1] == H and size[2] == 16 * E and sk[2] == sv[2] == 1 and dt == v.dtype == cache.tail.dtype
