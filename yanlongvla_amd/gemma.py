@@ -177,13 +177,14 @@ class KV8Cache:
         self.base = self.length = ks[0].shape[0]
         self.cap = self.base + room
         dev, D = ks[0].device, ks[0].shape[1]
-        self.start = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.start, self.end = (torch.zeros(1, dtype=torch.int32, device=dev) for _ in range(2))     # of the next row, after it
         self.caches = [kernels.kv8_cache(1, 1, D, self.cap, dev, k.dtype) for k in ks]
         for c, k, v in zip(self.caches, ks, vs):
             kernels.kv8_append(c, k.contiguous()[:, None], v.contiguous()[:, None], self.start)
         tail = self.base // kernels.KV8_BLOCK * kernels.KV8_BLOCK
         self.last = [(k[tail:].clone()[:, None], v[tail:].clone()[:, None]) for k, v in zip(ks, vs)]
         self.start.fill_(self.base)
+        self.end.fill_(self.base + 1)
 
     def rewind(self):
         from . import kernels
@@ -191,6 +192,7 @@ class KV8Cache:
         for c, (k, v) in zip(self.caches, self.last):
             kernels.kv8_append(c, k, v, tail)
         self.start.fill_(self.base)
+        self.end.fill_(self.base + 1)
         self.length = self.base
 
     def rows(self, i):
@@ -198,11 +200,12 @@ class KV8Cache:
         from . import kernels
         if self.length >= self.cap:
             raise RuntimeError(f'KV cache full ({self.length} rows)')
-        return kernels.KV8Rows(self.caches[i], self.start), None, None
+        return kernels.KV8Rows(self.caches[i], self.start, self.end), None, None
 
     def advance(self):
         self.length += 1
         self.start.add_(1)
+        self.end.add_(1)
 
 
 EXPERT = dict(layers=18, width=1024, hidden=4096, heads=8, head_dim=256, action_dim=32)

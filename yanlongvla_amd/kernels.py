@@ -525,9 +525,9 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
 
 class KV8Rows:
     """An 8-bit cache as a decoder layer takes it in the place of its key rows (gemma.KV8Cache.rows): the layer's KV8 of one sequence, the
-    position that this call's rows go to (start, (1,) int32 on the device) and, when `lens` is given, the length after them (else it is
-    made per call). core() appends the rows and attends over the whole: a later call with the same start replaces them, as long as they
-    are at most 64 (the action tokens of a denoising step)."""
+    position that this call's rows go to (start, (1,) int32 on the device) and, for calls of one row, the length after it (lens; it is
+    start plus the rows where it is not given). core() appends the rows and attends over the whole: a later call with the same start
+    replaces them, as long as they are at most 64 (the action tokens of a denoising step)."""
 
     def __init__(self, cache, start, lens=None, keys=None):
         self.cache, self.start, self.lens, self.keys = cache, start, lens, keys
@@ -536,7 +536,7 @@ class KV8Rows:
         """Attention of q (M, heads * D) after k, v (M, H * D): o (M, heads * D)."""
         M, D = q.shape[0], 16 * self.cache.k8.shape[4]
         kv8_append(self.cache, k.reshape(M, -1, D), v.reshape(M, -1, D), self.start)
-        lens = self.start + M if self.lens is None else self.lens
+        lens = self.start + M if self.lens is None or M > 1 else self.lens
         return kv8_attend(q.reshape(M, heads, D), self.cache, lens, causal=causal, keys=self.keys).view(M, heads * D)
 
 
