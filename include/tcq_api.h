@@ -314,7 +314,7 @@ int tcq_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int
 
 /* A key / value cache in 8 bits: B sequences, H KV heads of D = 64, 128 or 256, nblk blocks of TCQ_KV8_BLOCK tokens each. A block of a
  * head has one FP32 scale for its keys and one for its values, scale = max|x| / 127 over the rows that it holds (1 for zeros), codes
- * rint(x / scale). Infinities count as the block's largest code and NaN as 0: 8 bits have neither.
+ * rint(127 x / max|x|). Infinities count as the block's largest code and NaN as 0: 8 bits have neither.
  *   k8 (B, H, nblk, 4, D / 16, 16, 16) int8 = (token / 16, dim / 16, token % 16, dim % 16)
  *   v8 (B, H, nblk, D / 16, 4, 16, 16) int8 = (dim / 16, token % 16 / 4, dim % 16, token / 16 * 4 + token % 4)
  *   scale (B, H, nblk, 2) FP32 (keys, values); tail (B, H, 2, 2, 64, D) of the rows' type = (block % 2, keys | values, token, dim):

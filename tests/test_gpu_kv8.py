@@ -41,7 +41,8 @@ def values(x):
         f = torch.where(f.isnan(), torch.zeros_like(f), f)
         big = torch.where(f.isinf(), torch.zeros_like(f), f).abs().amax((0, 2), keepdim=True)
         s = torch.where(big > 0, big / torch.full_like(big, 127), torch.ones_like(big))      # (by a number, torch multiplies by 1 / 127)
-        out[j:j + T] = (torch.minimum(torch.maximum(f, -big), big) / s).round() * s
+        code = 127 * torch.minimum(torch.maximum(f, -big), big).double() / torch.where(big > 0, big, torch.ones_like(big)).double()
+        out[j:j + T] = code.round().float() * s
     return out
 
 
@@ -144,6 +145,25 @@ def test_appends_and_rows_taken_back_at_random(seed):
     K.kv8_append(one, k[:end], v[:end], ints([0]))
     got, want = ([x[0] for x in K.kv8_read(c, ints([0]), ints([end]), end, FP)] for c in (cache, one))
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize('dt', [BF, HF])
+def test_half_of_the_largest_is_a_tie(dt):
+    """Blocks of +-(largest, half of it), whatever the largest's rounded scale: code 127 and, half to even, 64. Largest values from the
+    types' smallest to their greatest ones."""
+    from yanlongvla_amd import kernels as K
+    n, fi = 300, torch.finfo(dt)
+    most = torch.logspace(math.log2(fi.smallest_normal), math.log2(fi.max), n, 2, dtype=torch.float64, device=DEV).clamp(max=fi.max).to(dt)
+    most[:4] = torch.tensor([2.0, 4.0, 6.0, 254.0], device=DEV).to(dt) * fi.smallest_normal * fi.eps     # denormal ones
+    half = most / 2
+    x = torch.zeros(n * T, 1, 64, dtype=dt, device=DEV)
+    x[::T, 0, 0], x[5::T, 0, 7], x[63::T, 0, 63] = 2 * half, half, -half
+    cache = K.kv8_cache(1, 1, 64, n * T, DEV, dt)
+    K.kv8_append(cache, x, x, ints([0]))
+    codes = cache.k8[0, 0].permute(0, 1, 3, 2, 4).reshape(n, T, 64)
+    assert (codes[:, 0, 0] == 127).all() and (codes[:, 5, 7] == 64).all() and (codes[:, 63, 63] == -64).all()
+    got = K.kv8_read(cache, ints([0]), ints([n * T]), n * T, FP)
+    assert all(torch.equal(y[0], values(x)) for y in got)
 
 
 def test_views_other_sequences_and_the_capacity():

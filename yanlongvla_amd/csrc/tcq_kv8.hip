@@ -112,7 +112,11 @@ __global__ __launch_bounds__(4 * D) void k_kv8_append(KvAppend a) {
     }
     const float sc = token_scale(amax);
     u32 w[4];
-    q8_words<4>(v, qscale(sc), w);
+    // the code is rint(127 x / amax), both sides by 128: a 16-bit value times 127 is exact, so a value of half the largest is the tie that it is
+    // (over the rounded scale it would fall to either side)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= 127.f / 128.f;
+    q8_words<4>(v, qscale(amax > 0.f ? amax * 0x1p-7f : 1.f), w);
     const size_t at = bh * a.nblk + blk;
     if (tid == 0) a.scale[at * 2 + val] = sc;
     const int unit = val ? (d / 16 * 4 + t / 4) * 16 + d % 16 : tid;
