@@ -1,11 +1,12 @@
 // Rotary positions with several axes (time, height, width): pair i of a head turns by pos[axis[i]] * freq[i].
 //
 // The angle is taken in turns in FP64 (pos * freq / 2 pi, minus its nearest whole number) and only then rounded to FP32: at
-// position 100000 an FP32 product is off by 4e-3 rad, this one by 1e-11 before the FP32 rounding of a number below one half. A
-// workgroup computes the cosines and sines of its tokens once, into LDS, while the loads of its rows are in flight; every
-// head of the token then uses them. MI355X: 4761 tokens of 32 heads x 64, FP32, 13.8 us (78 MB, 5.7 TB/s, some of it out of the
-// last-level cache: memory bound), 2048 tokens of 24 heads x 128, BF16, 7.7 us (25 MB, 3.3 TB/s: launch, the FP64 angles and one wave of
-// loads per workgroup), one token of the same 2.7 us.
+// position 100000 an FP32 product is off by 4e-3 rad, this one by 1e-11 before the FP32 rounding of a number below one half (up to
+// 9e-8 rad: for FP32 rows what it cuts off is put back in first order, 4.1e-8 relative against 64 bits instead of 5.9e-8). A workgroup
+// computes the cosines and sines of its tokens once, into LDS, while the loads of its rows are in flight; every head of the token then
+// uses them. MI355X: 4761 tokens of 32 heads x 64, FP32, 13.8 us (78 MB, 5.7 TB/s, some of it out of the last-level cache: memory
+// bound), 2048 tokens of 24 heads x 128, BF16, 7.7 us (25 MB, 3.3 TB/s: launch, the FP64 angles and one wave of loads per workgroup),
+// one token of the same 2.7 us.
 #include "tcq_device.h"
 #include "tcq_launch.h"
 
@@ -60,6 +61,7 @@ __device__ __forceinline__ uint4_t rope_pack(const float (&v)[E]) {
 }
 
 // cosine and sine of the pairs of tokens t0 .. t0 + n - 1 into cs (n x R / 2); an axis outside 0 .. A - 1 turns by nothing
+template <int DT>
 __device__ __forceinline__ void rope_table(const RopeArgs& a, int t0, int n, float2_t* cs) {
     const int half = a.R >> 1;
     for (int i = threadIdx.x; i < n * half; i += RT) {
@@ -73,6 +75,11 @@ __device__ __forceinline__ void rope_table(const RopeArgs& a, int t0, int n, flo
         }
         float s, c;
         sincospif(2.f * (float)turns, &s, &c);
+        if constexpr (DT == TCQ_F32) {
+            const float e = (float)((turns - (double)(float)turns) * 6.283185307179586), c0 = c;
+            c = __builtin_fmaf(-s, e, c);
+            s = __builtin_fmaf(c0, e, s);
+        }
         cs[i] = float2_t{c, a.inverse ? -s : s};
     }
 }
@@ -111,7 +118,7 @@ __global__ __launch_bounds__(RT) void k_rope(RopeArgs a, int TT) {
         }
     };
     load();
-    rope_table(a, t0, n, cs);
+    rope_table<DT>(a, t0, n, cs);
     __syncthreads();
     for (;;) {
 #pragma unroll
@@ -168,7 +175,7 @@ __global__ __launch_bounds__(RT) void k_rope_any(RopeArgs a, int adj) {
         part.freq += f0;
         if (part.axis) part.axis += f0;
         __syncthreads();
-        rope_table(part, t, 1, cs);
+        rope_table<DT>(part, t, 1, cs);
         __syncthreads();
         for (int u = threadIdx.x; u < H * nf; u += RT) {
             const int h = u / nf, f = u - h * nf;
