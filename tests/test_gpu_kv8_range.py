@@ -1,0 +1,94 @@
+"""GPU tests of the attention over the 8-bit cache at the ends of its range, against 64 bits over the values that the cache stands for: large
+scores, blocks of one large and many small probabilities, value scales far apart or denormal, lengths past the capacity.
+
+Tolerance, 2-norm of the difference over that of the result: half a step of the output type (2^-8 BF16, 2^-11 FP16), plus 2e-4 for the
+query's and the probabilities' 16-bit integers (a probability is off by 1 / 65278 of its block's largest; the queries' share is stated where it is
+larger)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+T = 64
+
+
+@pytest.fixture(scope='module', autouse=True)
+def _lib():
+    from yanlongvla_amd import _lib
+    _lib.lib()
+    torch.cuda.init()
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def rand(*shape, seed, dt=FP):
+    return torch.randn(*shape, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).to(dt)
+
+
+def fill(B, n, H, D, dt=BF, seed=0):
+    """A cache of B sequences of n normal rows each."""
+    from yanlongvla_amd import kernels as K
+    cache = K.kv8_cache(B, H, D, n, DEV, dt)
+    K.kv8_append(cache, rand(B * n, H, D, seed=seed, dt=dt), rand(B * n, H, D, seed=seed + 1, dt=dt), ints([0] * B))
+    return cache
+
+
+def held(cache, n):
+    """The values that a cache stands for, k and v (B, n, H, D) in 64 bits: codes times scales (in 32 bits the smallest ones would round)."""
+    B, H, N, _, E = cache.k8.shape[:5]
+    k = cache.k8.permute(0, 1, 2, 3, 5, 4, 6).reshape(B, H, N * T, E * 16)
+    v = cache.v8.view(B, H, N, E, 4, 16, 4, 4).permute(0, 1, 2, 6, 4, 7, 3, 5).reshape(B, H, N * T, E * 16)
+    s = cache.scale.double().repeat_interleave(T, 2)
+    return [(x.double() * s[..., i:i + 1]).transpose(1, 2)[:, :n] for i, x in enumerate((k, v))]
+
+
+def reference(q, k, v, lens, G, causal=False, scale=None):
+    """FP64 attention of len(lens) equal shares of the rows q over k, v (B, n, H, D)."""
+    m, out = q.shape[0] // len(lens), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    for b, n in enumerate(lens):
+        rows = slice(b * m, b * m + m)
+        for h in range(q.shape[1]):
+            s = q[rows, h].double() @ k[b, :n, h // G].t() * (scale or 1 / math.sqrt(q.shape[2]))
+            if causal:
+                s = s.masked_fill(torch.arange(n, device=q.device)[None] > torch.arange(m, device=q.device)[:, None] + n - m, -math.inf)
+            out[rows, h] = torch.softmax(s, 1) @ v[b, :n, h // G]
+    return out
+
+
+def close(o, want, more=0.0):
+    tol = torch.finfo(o.dtype).eps / 2 + 2e-4 + more
+    assert torch.isfinite(o).all()
+    assert (o.double() - want).norm() <= tol * want.norm()
+
+
+def each_row_close(o, want, more=0.0):
+    """The same for every row and head alone."""
+    tol = torch.finfo(o.dtype).eps / 2 + 2e-4 + more
+    assert torch.isfinite(o).all()
+    assert ((o.double() - want).norm(dim=-1) <= tol * want.norm(dim=-1)).all()
+
+
+# one launch of eight waves, four waves in parts, four waves with 64 dims, two row tiles a wave with 128 and 64 dims
+FORMS = [(2, 16, 8, 1, 256, 300), (2, 16, 8, 1, 256, 3000), (1, 40, 4, 2, 64, 1500), (2, 600, 16, 8, 128, 700), (4, 600, 16, 8, 64, 300)]
+
+
+@pytest.mark.parametrize('dt', [BF, HF])
+@pytest.mark.parametrize('logit', [100.0, 400.0, 700.0, 1500.0, 5000.0, 1e5])
+@pytest.mark.parametrize('B,M,Hq,Hk,D,n', FORMS)
+def test_large_scores_pick_their_key(B, M, Hq, Hk, D, n, logit, dt):
+    """Every query row is a multiple of one key, whose score is `logit`, several standard deviations above the others': the
+    output is that key's value."""
+    from yanlongvla_amd import kernels as K
+    logit = min(logit, 1e5 if dt == BF else 1e4)                       # (FP16 queries end at 65504)
+    cache = fill(B, n, Hk, D, dt, seed=11)
+    k, v = held(cache, n)
+    pick = torch.randint(0, n, (B, M, Hq), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    b, h = torch.arange(B, device=DEV)[:, None, None], torch.arange(Hq, device=DEV) // (Hq // Hk)
+    key = k[b, pick, h]                                                # (B, M, Hq, D)
+    q = (key * (logit * D ** 0.5 / key.square().sum(-1, keepdim=True))).to(dt).view(B * M, Hq, D)
+    each_row_close(K.kv8_attend(q, cache, ints([n] * B), causal=False), v[b, pick, h].view(B * M, Hq, D))

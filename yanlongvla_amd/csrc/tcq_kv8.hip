@@ -463,8 +463,9 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
             const float mb = none ? 0.f : mx * c;
             float p[16], lb = 0.f;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[x], c, -mb));
-            if constexpr (edge)                                      // also where c is 0 and the product above NaN
+            for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f((f[x] - mx) * c);   // at most 1: the digits hold no more (mb is rounded,
+                                                                                            // f c - mb past zero from scores of some hundreds on)
+            if constexpr (edge)                                      // also where c is 0, or nothing visible, and the product above NaN
 #pragma unroll
                 for (int x = 0; x < 16; ++x) p[x] = left(0, x) ? p[x] : 0.f;
 #pragma unroll
