@@ -92,3 +92,19 @@ def test_large_scores_pick_their_key(B, M, Hq, Hk, D, n, logit, dt):
     key = k[b, pick, h]                                                # (B, M, Hq, D)
     q = (key * (logit * D ** 0.5 / key.square().sum(-1, keepdim=True))).to(dt).view(B * M, Hq, D)
     each_row_close(K.kv8_attend(q, cache, ints([n] * B), causal=False), v[b, pick, h].view(B * M, Hq, D))
+
+
+def test_weights_of_a_block_add_up_to_one():
+    """One key of a block ahead of 63 whose probabilities are 0.489 of a digit each, values that are all 1: the output is 1, whatever the small
+    probabilities are rounded to. Numerator and denominator are the same whole numbers times powers of two and the value's 127 / 127: three
+    FP32 roundings, then the type's half step."""
+    from yanlongvla_amd import kernels as K
+    for D, n in ((64, 64), (256, 64), (128, 128)):
+        k = torch.zeros(n, 1, D, dtype=HF, device=DEV)
+        k[::T, 0, 0] = 1                                               # the only key that counts, one in every block
+        cache = K.kv8_cache(1, 1, D, n, DEV, HF)
+        K.kv8_append(cache, k, torch.ones_like(k), ints([0]))
+        q = torch.zeros(3, 1, D, dtype=HF, device=DEV)
+        q[:, 0, 0] = 11.109 * D ** 0.5                                 # exp(-11.109) = 0.489 / 32639
+        o = K.kv8_attend(q, cache, ints([n]), causal=False)
+        assert ((o.double() - 1).abs() <= 2.0 ** -11 + 4 * 2.0 ** -24).all()

@@ -461,21 +461,25 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
             const float mx = across(largest(0));
             const bool none = edge && mx == -__builtin_inff();       // the row sees no key of the block
             const float mb = none ? 0.f : mx * c;
-            float p[16], lb = 0.f;
+            float p[16];
 #pragma unroll
             for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f((f[x] - mx) * c);   // at most 1: the digits hold no more (mb is rounded,
                                                                                             // f c - mb past zero from scores of some hundreds on)
             if constexpr (edge)                                      // also where c is 0, or nothing visible, and the product above NaN
 #pragma unroll
                 for (int x = 0; x < 16; ++x) p[x] = left(0, x) ? p[x] : 0.f;
+            // the sum of the rounded probabilities, which are the weights that the values get: whole numbers in the low bits of p + DIG
+            u32 lb = -16u * __float_as_uint(DIG);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) lb += p[x];
+            for (int x = 0; x < 16; ++x) {
+                p[x] = __builtin_fmaf(p[x], PC, DIG);
+                lb += __float_as_uint(p[x]);
+            }
             uint4_t Ph, Pl;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 u32 h4, l4;
-                digits(__builtin_fmaf(p[4 * x], PC, DIG), __builtin_fmaf(p[4 * x + 1], PC, DIG), __builtin_fmaf(p[4 * x + 2], PC, DIG),
-                       __builtin_fmaf(p[4 * x + 3], PC, DIG), h4, l4);
+                digits(p[4 * x], p[4 * x + 1], p[4 * x + 2], p[4 * x + 3], h4, l4);
                 Ph[x] = h4;
                 Pl[x] = l4;
             }
@@ -488,7 +492,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 mr[0] = up ? mb : mr[0];
             }
             const float w = none ? 0.f : __builtin_amdgcn_exp2f(mb - mr[0]), be = none ? 0.f : w * (svj * (1.f / PC));
-            l[0] = __builtin_fmaf(w, lb, l[0]);
+            l[0] = __builtin_fmaf(w * (1.f / PC), (float)(int)lb, l[0]);
 #pragma unroll
             for (int dt = 0; dt < DTL; ++dt) {
                 const int4_t z = {0, 0, 0, 0};
