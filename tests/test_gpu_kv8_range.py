@@ -48,7 +48,7 @@ def held(cache, n):
 
 
 def reference(q, k, v, lens, G, causal=False, scale=None):
-    """FP64 attention of len(lens) equal shares of the rows q over k, v (B, n, H, D)."""
+    """FP64 attention of len(lens) equal shares of the rows q over k, v (B, n, H, D); a row that sees nothing is zeros."""
     m, out = q.shape[0] // len(lens), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     for b, n in enumerate(lens):
         rows = slice(b * m, b * m + m)
@@ -56,7 +56,7 @@ def reference(q, k, v, lens, G, causal=False, scale=None):
             s = q[rows, h].double() @ k[b, :n, h // G].t() * (scale or 1 / math.sqrt(q.shape[2]))
             if causal:
                 s = s.masked_fill(torch.arange(n, device=q.device)[None] > torch.arange(m, device=q.device)[:, None] + n - m, -math.inf)
-            out[rows, h] = torch.softmax(s, 1) @ v[b, :n, h // G]
+            out[rows, h] = torch.nan_to_num(torch.softmax(s, 1), nan=0.0) @ v[b, :n, h // G]
     return out
 
 
@@ -108,3 +108,26 @@ def test_weights_of_a_block_add_up_to_one():
         q[:, 0, 0] = 11.109 * D ** 0.5                                 # exp(-11.109) = 0.489 / 32639
         o = K.kv8_attend(q, cache, ints([n]), causal=False)
         assert ((o.double() - 1).abs() <= 2.0 ** -11 + 4 * 2.0 ** -24).all()
+
+
+ROWS = [(2, 600, 16, 8, 128, 700), (4, 600, 16, 8, 64, 300)]           # two row tiles a wave
+
+
+@pytest.mark.parametrize('B,M,Hq,Hk,D,n', ROWS)
+@pytest.mark.parametrize('causal', [False, True])
+def test_denormal_value_scales_of_many_rows(B, M, Hq, Hk, D, n, causal):
+    """BF16 values whose scale is denormal in FP32 in some blocks, in all of them, or in none of those that a row sees."""
+    from yanlongvla_amd import kernels as K
+    cache = fill(B, n, Hk, D, seed=21)
+    q = rand(B * M, Hq, D, seed=22, dt=BF) * 2
+    for blocks in (slice(1, 2), slice(0, 1), slice(None)):
+        scale = cache.scale.clone()
+        scale[:, :, blocks, 1] *= 2.0 ** -122                          # about 2^-127 to 2^-128
+        assert (scale[:, :, blocks, 1] < torch.finfo(FP).smallest_normal).all() and (scale > 0).all()
+        big = cache._replace(scale=scale)
+        o = K.kv8_attend(q, big, ints([n] * B), causal=causal)
+        want = reference(q, *held(big, n), [n] * B, Hq // Hk, causal)
+        if blocks == slice(None):                                      # a result of 2^-122 to 2^-127 rounds to whole multiples of 2^-133
+            assert ((o.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2e-4 * want.abs().max() + 2.0 ** -134).all()
+        else:
+            close(o, want)

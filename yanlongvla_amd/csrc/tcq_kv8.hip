@@ -511,7 +511,8 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 er = ne;
             }
             // p sv = 2^(s - m + lu) rho; their sum in units of the probabilities is iu times what the MFMA adds
-            const float lu = __builtin_amdgcn_logf(svj) - (float)er, iu = __builtin_amdgcn_exp2f(-lu);
+            // (the logarithm of the mantissa: that of a denormal scale itself would be taken as one of zero)
+            const float lu = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(svj)) + (float)(es - er), iu = __builtin_amdgcn_exp2f(-lu);
             half8_t P[RT][2], ones;
 #pragma unroll
             for (int x = 0; x < 8; ++x) ones[x] = (_Float16)1.f;
