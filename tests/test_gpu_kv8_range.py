@@ -131,3 +131,24 @@ def test_denormal_value_scales_of_many_rows(B, M, Hq, Hk, D, n, causal):
             assert ((o.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2e-4 * want.abs().max() + 2.0 ** -134).all()
         else:
             close(o, want)
+
+
+@pytest.mark.parametrize('dt', [BF, HF])
+@pytest.mark.parametrize('Hq,Hk,D', [(16, 8, 128), (16, 16, 64)])
+def test_many_small_probabilities_behind_large_values(Hq, Hk, D, dt):
+    """32768 keys of one small probability each (2^-17.4 of the four keys' that are picked) behind blocks whose value scale is 50 times
+    theirs, values of opposite sign: together they are 4 % of the weight. As FP16 numbers in units of the larger scale they are 190 steps
+    of the smallest FP16 number, off by half of one: 2.6e-3 of 4 %, twice (both signs), 2.3e-4 in all."""
+    from yanlongvla_amd import kernels as K
+    M, n = 1024, 32768
+    k, v = (torch.zeros(n, Hk, D, dtype=dt, device=DEV) for _ in range(2))
+    v -= 1
+    k[:4 * T:T, :, 0] = 1
+    v[:4 * T:T] = 1
+    v[1:4 * T:T] = 50
+    cache = K.kv8_cache(1, Hk, D, n, DEV, dt)
+    K.kv8_append(cache, k, v, ints([0]))
+    q = torch.zeros(M, Hq, D, dtype=dt, device=DEV)
+    q[..., 0] = 12.086 * D ** 0.5
+    o = K.kv8_attend(q, cache, ints([n]), causal=False)
+    each_row_close(o, reference(q[:1], *held(cache, n), [n], Hq // Hk).expand(M, Hq, D), more=2.3e-4)

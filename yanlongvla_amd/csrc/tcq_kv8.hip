@@ -235,6 +235,7 @@ struct KvAttend {
 
 constexpr float QC = 32512.f;    // query digits: 127 * 256, the largest value whose rounded high digit stays within 127
 constexpr float PC = 32639.f;    // probability digits: 127 * 256 + 127
+constexpr int UP = 7;            // FP16 probabilities are raised by 2^7: up to 2^8 before the outputs are rescaled, so up to 2^15 of FP16's 2^16
 constexpr float DIG = 12582912.f + 128.f;   // 1.5 * 2^23 + 128: adding it leaves the rounded integer plus 128 in the low bits
 
 // four values as two words of INT8 digits: value = 256 hi + lo, lo in [-128, 127]. f: value + DIG
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     const uint4_t* Q = (const uint4_t*)lds + lane;                   // digits hi, lo of K step ks of tile rt at 128 (KS rt + ks), + 64
     float4_t O[RT][DTL];
     float mr[RT], l[RT], top = 0.f;
-    int er = -126;                                                   // RT > 1: rho = 2^er
+    int er = -126;                                                   // RT > 1: rho = 2^(er - UP)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         mr[rt] = -__builtin_inff();
@@ -510,9 +511,9 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 shift = er - ne;
                 er = ne;
             }
-            // p sv = 2^(s - m + lu) rho; their sum in units of the probabilities is iu times what the MFMA adds
+            // p sv = 2^(s - m + lu) 2^(er - UP); their sum in units of the probabilities is iu times what the MFMA adds
             // (the logarithm of the mantissa: that of a denormal scale itself would be taken as one of zero)
-            const float lu = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(svj)) + (float)(es - er), iu = __builtin_amdgcn_exp2f(-lu);
+            const float lu = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(svj)) + (float)(es - er + UP), iu = __builtin_amdgcn_exp2f(-lu);
             half8_t P[RT][2], ones;
 #pragma unroll
             for (int x = 0; x < 8; ++x) ones[x] = (_Float16)1.f;
@@ -562,7 +563,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     constexpr int WD = DTL < W ? DTL : W, DW = DTL / WD;             // waves that sum, dim tiles of each
     float4_t* x = (float4_t*)lds;
     float *sm = (float*)(lds + W * DTL * 1024), *sl = sm + 16 * W;
-    const float rho = RT == 1 ? 1.f : __builtin_amdgcn_ldexpf(1.f, er);
+    const float rho = RT == 1 ? 1.f : __builtin_amdgcn_ldexpf(1.f, er - UP);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         __syncthreads();
