@@ -152,3 +152,43 @@ def test_many_small_probabilities_behind_large_values(Hq, Hk, D, dt):
     q[..., 0] = 12.086 * D ** 0.5
     o = K.kv8_attend(q, cache, ints([n]), causal=False)
     each_row_close(o, reference(q[:1], *held(cache, n), [n], Hq // Hk).expand(M, Hq, D), more=2.3e-4)
+
+
+@pytest.mark.parametrize('order', [(0, 1), (1, 0), (0, 0, 1), (1, 1, 1, 1, 1, 0)])
+@pytest.mark.parametrize('e', [(0, -100), (100, 0), (60, -60), (0, -120), (3, -12)])
+@pytest.mark.parametrize('B,M,Hq,Hk,D,n', [*ROWS, (2, 16, 16, 8, 128, 700)])
+def test_value_scales_far_apart(B, M, Hq, Hk, D, n, e, order):
+    """Two kinds of blocks in turn whose value scales differ by up to 2^120; every other row (token and head) looks at the one kind alone, the rest at
+    the other (the scores lie 170 apart): each row for itself is held to 64 bits, whatever the other rows of its tile look at.
+    The queries' largest value is 32: a digit is off by 32 / 32512 / sqrt(12) root mean square, keys of norm sqrt(D + 8 * 16), scale 1 / sqrt(D):
+    4e-4, taken twice for single rows."""
+    from yanlongvla_amd import kernels as K
+    cache = fill(B, n, Hk, D, seed=31)
+    k8, scale = cache.k8.clone(), cache.scale.clone()
+    for j in range(k8.shape[2]):
+        kind = order[j % len(order)]
+        k8[:, :, j, :, 0, :, :8] = 127 if kind else -127
+        scale[:, :, j, 1] *= 2.0 ** e[kind]
+    big = K.KV8(k8, cache.v8, scale, cache.tail)
+    q = rand(B * M, Hq, D, seed=32)
+    sign = 1 - 2 * ((torch.arange(B * M, device=DEV)[:, None] + torch.arange(Hq, device=DEV)) % 2)
+    q[..., :8] = 30.0 * sign[..., None]
+    q = q.to(BF)
+    o = K.kv8_attend(q, big, ints([n] * B), causal=False)
+    each_row_close(o, reference(q, *held(big, n), [n] * B, Hq // Hk), more=2 * 32 / 32512 / 12 ** 0.5 * ((D + 128) / D) ** 0.5)
+
+
+@pytest.mark.parametrize('B,M,Hq,Hk,D,n', ROWS)
+@pytest.mark.parametrize('causal', [False, True])
+def test_blocks_of_zeros_among_small_values(B, M, Hq, Hk, D, n, causal):
+    """A block of zero values has scale 1, others 2^-100 of a usual one; and a scale of zero, which counts as zeros."""
+    from yanlongvla_amd import kernels as K
+    cache = fill(B, n, Hk, D, seed=41)
+    q = rand(B * M, Hq, D, seed=42, dt=BF)
+    for zero in (1.0, 0.0):
+        v8, scale = cache.v8.clone(), cache.scale.clone()
+        scale[..., 1] *= 2.0 ** -100
+        v8[:, :, 1::3] = 0
+        scale[:, :, 1::3, 1] = zero
+        big = K.KV8(cache.k8, v8, scale, cache.tail)
+        close(K.kv8_attend(q, big, ints([n] * B), causal=causal), reference(q, *held(big, n), [n] * B, Hq // Hk, causal))

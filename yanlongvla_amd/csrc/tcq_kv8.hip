@@ -280,10 +280,11 @@ __device__ __forceinline__ void widen(uint4_t w, half8_t& a, half8_t& b) {
 //                 (m the block's own maximum: a block whose probabilities are all small keeps its digits), exact int32 sums that are
 //                 scaled and added in FP32: nothing is converted, but every output is touched once a block.
 //                 RT > 1: FP16, A = 16 dims x 32 keys widened in registers (two instructions for two values, for all RT tiles: the byte as
-//                 the low half of 1024 + 128 + code, less 1152, exact), B = the probabilities times the block's value scale / rho, FP32
-//                 sums that stay in the accumulators in units of rho, a power of two near the block's scale (the scale rides on the
-//                 exponent; a unit that changes rescales them exactly, down to 2^-60 of the largest scale so far); the probabilities' sum
-//                 is their product with ones.
+//                 the low half of 1024 + 128 + code, less 1152, exact), B = the probabilities times the block's value scale / 2^u, FP32
+//                 sums that stay in the accumulators in units of 2^u, which every row has of its own, 2^-7 of a block's scale (the scale
+//                 rides on the exponent; a unit that changes rescales the row's sums exactly); the probabilities' sum is their product
+//                 with ones. Where the scales of a row's blocks lie so far apart that no unit holds both its sums and the block, the sum
+//                 takes the probabilities all the same and the values' products are left at what FP16 has of them.
 // The outputs are rescaled only once a maximum is a factor of 256 past the one that they stand on.
 // A wave holds one block's keys or values at a time and leaves the overlap of loads, matrix and vector instructions to the other waves of
 // its SIMD (four of them for D up to 128): one wave issues a vector instruction every 7 to 13 cycles here, four together every 3 to 5. With
@@ -410,12 +411,12 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     local_barrier();
     const uint4_t* Q = (const uint4_t*)lds + lane;                   // digits hi, lo of K step ks of tile rt at 128 (KS rt + ks), + 64
     float4_t O[RT][DTL];
-    float mr[RT], l[RT], top = 0.f;
-    int er = -126;                                                   // RT > 1: rho = 2^(er - UP)
+    float mr[RT], l[RT], u[RT];                                      // u: RT > 1, the row's outputs are in units of 2^u
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         mr[rt] = -__builtin_inff();
         l[rt] = 0.f;
+        u[rt] = -160.f;                                              // (below every scale's)
 #pragma unroll
         for (int dt = 0; dt < DTL; ++dt) O[rt][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -502,39 +503,60 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 for (int e = 0; e < 4; ++e) O[0][dt][e] = __builtin_fmaf((float)((oh[e] << 8) + ol[e]), be, O[0][dt][e]);
             }
         } else {
-            // the unit of the outputs, changed when the scale leaves [unit / 64, unit]
-            int shift = 0;
-            const int es = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(svj));
-            if (es > er || es < er - 6) {                            // uniform
-                top = fmaxf(top, svj);
-                const int ne = max(min(es, 127), __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(top)) - 60);
-                shift = er - ne;
-                er = ne;
-            }
-            // p sv = 2^(s - m + lu) 2^(er - UP); their sum in units of the probabilities is iu times what the MFMA adds
-            // (the logarithm of the mantissa: that of a denormal scale itself would be taken as one of zero)
-            const float lu = __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(svj)) + (float)(es - er + UP), iu = __builtin_amdgcn_exp2f(-lu);
+            // the block's value scale 2^ls (the logarithm of the mantissa: that of a denormal scale itself would be taken as one of zero). A scale
+            // of zero, which no append makes, counts as the smallest one.
+            const float es = svj == 0.f ? -150.f : (float)__builtin_amdgcn_frexp_expf(svj);
+            const float ls = svj == 0.f ? es : es + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(svj));
             half8_t P[RT][2], ones;
 #pragma unroll
             for (int x = 0; x < 8; ++x) ones[x] = (_Float16)1.f;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 scores(rt);
-                float mx = largest(rt);
-                if (shift || __builtin_amdgcn_ballot_w64(mx * c > mr[rt] + 8.f)) {   // uniform
-                    mx = across(mx);
-                    const float mb = edge && mx == -__builtin_inff() ? mx : mx * c;
-                    const bool up = mb > mr[rt] + 8.f;
-                    const float al = up ? __builtin_amdgcn_exp2f(mr[rt] - mb) : 1.f, ak = __builtin_amdgcn_ldexpf(al, shift);
-                    l[rt] *= al;
+                const float mx = largest(rt);
+                // FP16 probabilities 2^(s - m + lu), whose products with the codes are in units of 2^u. (mr -inf: the row's first key)
+                float lu = ls - u[rt], mz = lu - mr[rt], g = 1.f;
+                bool cut = false;
+                if (__builtin_amdgcn_ballot_w64(__builtin_fmaf(mx, c, mz) > 15.f || lu < 0.f)) {   // uniform
+                    const float m0 = mr[rt], ma = across(mx), mb = edge && ma == -__builtin_inff() ? ma : ma * c;
+                    const bool up = mb > m0 + 8.f;
+                    const float down = up ? m0 - mb : 0.f;           // what the sums so far lie under the new maximum
+                    mr[rt] = up ? mb : m0;
+                    l[rt] *= __builtin_amdgcn_exp2f(down);
+                    // a unit for the block's largest product where that is past FP16, one for the block's scale where the probabilities
+                    // would fall out of it, as far as the outputs so far leave room for that (2^100)
+                    float n = u[rt];
+                    if (mb - mr[rt] + lu > 15.f) n = es - UP + fminf(__builtin_ceilf(mb - mr[rt]), 0.f);
+                    if (__builtin_amdgcn_ballot_w64(ls < n)) {       // uniform
+                        float mo = 0.f;
 #pragma unroll
-                    for (int dt = 0; dt < DTL; ++dt) O[rt][dt] *= ak;
-                    mr[rt] = up ? mb : mr[rt];
+                        for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mo = fmaxf(mo, fabsf(O[rt][dt][e]));
+                        mo = across(mo);
+                        const float room = mo > 0.f ? u[rt] + down + (float)(__builtin_amdgcn_frexp_expf(mo) - 100) : -__builtin_inff();
+                        n = ls < n ? fminf(n, fmaxf(es - UP, room)) : n;
+                    }
+                    const float y = fmaxf(u[rt] - n + down, -500.f), yi = __builtin_floorf(y), yf = __builtin_amdgcn_exp2f(y - yi);
+                    u[rt] = n;
+                    lu = ls - n;
+                    if (__builtin_amdgcn_ballot_w64(m0 != -__builtin_inff())) {           // uniform; else the outputs are zeros
+#pragma unroll
+                        for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) O[rt][dt][e] = __builtin_amdgcn_ldexpf(O[rt][dt][e] * yf, (int)yi);
+                    }
+                    cut = __builtin_amdgcn_ballot_w64(lu < 0.f);
+                    if (cut) {                                       // no room: the sum takes the probabilities all the same, the values'
+                        g = lu < 0.f ? __builtin_amdgcn_exp2f(lu - UP) : 1.f;       // products of those rows lie below 2^-60 of their outputs
+                        lu = lu < 0.f ? (float)UP : lu;
+                    }
+                    mz = lu - mr[rt];
                 }
-                const float mz = edge && mr[rt] == -__builtin_inff() ? 0.f : mr[rt] - lu;
+                if (edge && mr[rt] == -__builtin_inff()) mz = 0.f;
                 float p[16];
 #pragma unroll
-                for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[x], c, -mz));
+                for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(f[x], c, mz));
                 if constexpr (edge)
 #pragma unroll
                     for (int x = 0; x < 16; ++x) p[x] = left(rt, x) ? p[x] : 0.f;
@@ -542,7 +564,10 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
                 for (int x = 0; x < 16; ++x) P[rt][x >> 3][x & 7] = (_Float16)p[x];
                 float4_t s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[rt][0], float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[rt][1], s, 0, 0, 0);
-                l[rt] = __builtin_fmaf(s[0], iu, l[rt]);             // (the same in all four lane groups)
+                l[rt] = __builtin_fmaf(s[0], __builtin_amdgcn_exp2f(-lu), l[rt]);        // (the same in all four lane groups)
+                if (cut)                                             // uniform
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) P[rt][x >> 3][x & 7] *= (_Float16)g;
             }
 #pragma unroll
             for (int dt = 0; dt < DTL; ++dt) {
@@ -563,7 +588,6 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     constexpr int WD = DTL < W ? DTL : W, DW = DTL / WD;             // waves that sum, dim tiles of each
     float4_t* x = (float4_t*)lds;
     float *sm = (float*)(lds + W * DTL * 1024), *sl = sm + 16 * W;
-    const float rho = RT == 1 ? 1.f : __builtin_amdgcn_ldexpf(1.f, er - UP);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         __syncthreads();
@@ -577,7 +601,13 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
             sl[16 * wave + lr] = s;
         }
 #pragma unroll
-        for (int dt = 0; dt < DTL; ++dt) x[(wave * DTL + dt) * 64 + lane] = RT == 1 ? O[rt][dt] : O[rt][dt] * rho;
+        for (int dt = 0; dt < DTL; ++dt) {
+            float4_t y = O[rt][dt];
+            if (RT > 1)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_ldexpf(y[e], (int)u[rt]);
+            x[(wave * DTL + dt) * 64 + lane] = y;
+        }
         __syncthreads();
         const int r = row0 + 16 * rt + lr;
         if (wave >= WD || r >= nrows) continue;
