@@ -192,3 +192,26 @@ def test_blocks_of_zeros_among_small_values(B, M, Hq, Hk, D, n, causal):
         scale[:, :, 1::3, 1] = zero
         big = K.KV8(cache.k8, v8, scale, cache.tail)
         close(K.kv8_attend(q, big, ints([n] * B), causal=causal), reference(q, *held(big, n), [n] * B, Hq // Hk, causal))
+
+
+@pytest.mark.parametrize('B,M,Hq,Hk,D', [(1, 20, 8, 1, 256), (1, 20, 4, 2, 64), (2, 1200, 8, 8, 64)])
+@pytest.mark.parametrize('past', [0, 1, 12, 64, 1000])
+def test_causal_rows_past_the_capacity(B, M, Hq, Hk, D, past):
+    """Lengths past the capacity: rows that no longer fit are dropped, row i of n still sees positions j <= lens - n + i of what is held."""
+    from yanlongvla_amd import kernels as K
+    n = 1280 if M > 20 else 128
+    cache = fill(B, n, Hk, D, seed=51)
+    k, v = held(cache, n)
+    q = rand(B * M, Hq, D, seed=52, dt=BF)
+    lens = [n + past, n - 7][:B]
+    o = K.kv8_attend(q, cache, ints(lens))
+    want = torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    for b, x in enumerate(lens):
+        for h in range(Hq):
+            s = q[b * M:b * M + M, h].double() @ k[b, :, h // (Hq // Hk)].t() / D ** 0.5
+            hidden = torch.arange(n, device=DEV)[None] > torch.arange(M, device=DEV)[:, None] + x - M
+            s = s.masked_fill(hidden | (torch.arange(n, device=DEV) >= x), -math.inf)
+            want[b * M:b * M + M, h] = torch.nan_to_num(torch.softmax(s, 1), nan=0.0) @ v[b, :, h // (Hq // Hk)]
+    close(o, want)
+    both = K.kv8_attend(q, cache, ints(lens), causal=False)              # every row sees what is held
+    close(both, reference(q, k, v, [min(x, n) for x in lens], Hq // Hk))

@@ -305,10 +305,10 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
     const int split = blockIdx.x % a.S, h = blockIdx.x / a.S, b = blockIdx.y, tile = a.last - blockIdx.z;
     const int c0 = a.cu ? max(0, a.cu[b]) : b * a.most, count = a.cu ? a.cu[b + 1] - c0 : a.most;
     const int m = min(min(count, a.most), a.rows - c0);              // rows computed here
-    const int L = min(max(a.lens[b], 0), a.nblk * KB);
+    const int n = max(a.lens[b], 0), L = min(n, a.nblk * KB);        // the length, which may go past the capacity, and what is held of it
     const int nrows = m * a.G, row0 = 16 * RT * tile;
     if (row0 >= nrows) return;                                       // uniform
-    auto sees = [&](int tt) { return a.causal ? min(max(L - count + tt + 1, 0), L) : L; };
+    auto sees = [&](int tt) { return a.causal ? min(max(n - count + tt + 1, 0), L) : L; };
     auto token = [&](int r, int& hq) {                               // row r of the KV head: its token and query head
         const int t = r / a.G;
         hq = h * a.G + (r - t * a.G);
