@@ -215,3 +215,16 @@ def test_causal_rows_past_the_capacity(B, M, Hq, Hk, D, past):
     close(o, want)
     both = K.kv8_attend(q, cache, ints(lens), causal=False)              # every row sees what is held
     close(both, reference(q, k, v, [min(x, n) for x in lens], Hq // Hk))
+
+
+@pytest.mark.parametrize('B,M,Hq,Hk,D,n', FORMS)
+@pytest.mark.parametrize('qe,ke', [(1e34, 1e-36), (1e36, 1e-37), (1e-36, 1e34), (1e-10, 1e10)])
+def test_huge_queries_of_tiny_keys(B, M, Hq, Hk, D, n, qe, ke):
+    """Scores of usual size from a product of very large and very small numbers."""
+    from yanlongvla_amd import kernels as K
+    cache = fill(B, n, Hk, D, seed=61)
+    scale = cache.scale.clone()
+    scale[..., 0] *= ke
+    big = cache._replace(scale=scale)
+    q = (rand(B * M, Hq, D, seed=62) * 2 * qe).to(BF)
+    close(K.kv8_attend(q, big, ints([n] * B), causal=False), reference(q, *held(big, n), [n] * B, Hq // Hk))

@@ -425,7 +425,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
         const float svj = sv;
         float c, f[16];                                              // one tile's scores at a time
         auto scores = [&](int rt) {
-            c = __builtin_amdgcn_ldexpf(qs[rt] * sk, E[rt]);
+            c = __builtin_amdgcn_ldexpf(sk, E[rt]) * qs[rt];         // (the scales first: one may be huge where the other is tiny)
             int4_t hi[4], lo[4];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
