@@ -850,11 +850,11 @@ extern "C" int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int 
             a.last = (int)(left - 1);                                                                                   \
             if (plan.W == 8) launch_k(k_kv8_attend<N, 8, 1>, grid, dim3(512), lds, st, a);                              \
             else if (N == 256 || plan.RT == 1) launch_k(k_kv8_attend<N, 4, 1>, grid, dim3(256), lds, st, a);            \
-            else launch_k(k_kv8_attend<N == 64 ? 64 : 128, 4, 2>, grid, dim3(256), lds, st, a);                             \
-        }                                                                                                               \
-        if (S > 1) {                                                                                                    \
+            else launch_k(k_kv8_attend<N == 64 ? 64 : 128, 4, 2>, grid, dim3(256), lds, st, a);                         \
             const int e = launch_status();                                                                              \
             if (e) return e;                                                                                            \
+        }                                                                                                               \
+        if (S > 1) {                                                                                                    \
             constexpr int PR = KT / (N / 4);                                                                            \
             if (S > 8) launch_k(k_kv8_join<N>, dim3((u32)most * Hq, 1, B), dim3(JT), 0, st, a);                         \
             else launch_k(k_kv8_join_few<N>, dim3(((u32)most * Hq + PR - 1) / PR, 1, B), dim3(KT), 0, st, a);             \
