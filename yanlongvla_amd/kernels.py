@@ -526,8 +526,9 @@ def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=No
 class KV8Rows:
     """An 8-bit cache as a decoder layer takes it in the place of its key rows (gemma.KV8Cache.rows): the layer's KV8 of one sequence, the
     position that this call's rows go to (start, (1,) int32 on the device) and, for calls of one row, the length after it (lens; it is
-    start plus the rows where it is not given). core() appends the rows and attends over the whole: a later call with the same start
-    replaces them, as long as they are at most 64 (the action tokens of a denoising step)."""
+    start plus the rows where it is not given). core() appends the rows, at most 64, and attends over the whole: a later call with the same
+    start replaces them (the action tokens of a denoising step). More rows would overwrite the 16-bit rows that the start's block is made of
+    again and are refused; rows that stay, like a prompt's, go through kv8_append and kv8_attend in any number."""
 
     def __init__(self, cache, start, lens=None, keys=None):
         self.cache, self.start, self.lens, self.keys = cache, start, lens, keys
@@ -535,6 +536,8 @@ class KV8Rows:
     def core(self, q, k, v, heads, causal):
         """Attention of q (M, heads * D) after k, v (M, H * D): o (M, heads * D)."""
         M, D = q.shape[0], 16 * self.cache.k8.shape[4]
+        if M > KV8_BLOCK:
+            raise ValueError(f'KV8Rows: {M} rows, at most {KV8_BLOCK} can be replaced by a later call (kv8_append and kv8_attend take more)')
         kv8_append(self.cache, k.reshape(M, -1, D), v.reshape(M, -1, D), self.start)
         lens = self.start + M if self.lens is None or M > 1 else self.lens
         return kv8_attend(q.reshape(M, heads, D), self.cache, lens, causal=causal, keys=self.keys).view(M, heads * D)
