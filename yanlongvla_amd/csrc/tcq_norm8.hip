@@ -60,8 +60,8 @@ __device__ __forceinline__ void n8_round(float (&v)[8], uint4_t (&w)[DT == TCQ_F
 // zero then), has scale 1 and codes 0.
 __device__ __forceinline__ void n8_scales(float sum, float big, float bad, float eps, int K, float& scale, float& step) {
     const float rms = 1.f / __builtin_sqrtf(sum / (float)K + eps), s = big * rms / 127.f;
-    const bool none = !(s > 0.f);
-    scale = bad != 0.f || __builtin_isnan(s) ? __builtin_nanf("") : none ? 1.f : s;
+    const bool none = big == 0.f || !(s > 0.f);                           // (zeros without an eps: s is 0 / 0)
+    scale = bad != 0.f || (big > 0.f && __builtin_isnan(s)) ? __builtin_nanf("") : none ? 1.f : s;
     step = none ? __builtin_inff() : big / 127.f;
 }
 // the two words of 8 codes of columns k .. k + 7
