@@ -270,7 +270,7 @@ def post_add_norm_pre(acc, s, rs, sv, bias, x, xout, w=None, eps=0.0, su=None, q
 def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offset=1.0):
     """h = x + r (r None: x), rounded to x's type and stored in xout where that is given (it may be x or r), then INT8 rows of
     RMSNorm(h) * (offset + w): q (M, K) int8 and / or q4 (as in pre), scale (M,) FP32, what gemm_i8 takes. x, r, xout (M, K) BF16 / FP16
-    / FP32 with contiguous rows of any stride, w (K,) of that type; offset 1: Gemma's weights, 0: plain ones."""
+    / FP32 with contiguous rows of any stride (xout's may not overlap), w (K,) of that type; offset 1: Gemma's weights, 0: plain ones."""
     size, dt = x.shape, x.dtype
     M, K = size
     if dt not in DTYPE or dt not in (torch.bfloat16, torch.float16, torch.float32):
@@ -278,6 +278,8 @@ def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offs
     for t in (x, r, xout):
         if t is not None and not (t.shape == size and t.dtype == dt and (t.stride(1) == 1 or K == 1)):
             raise ValueError(f'add_norm_quantize: x, r and xout must be ({M}, {K}) {dt} with contiguous rows')
+    if xout is not None and not _apart(M, 1, K, xout.stride(0), 0):
+        raise ValueError('add_norm_quantize: rows of xout overlap')
     if w.dtype != dt or w.numel() != K or not w.is_contiguous():
         raise ValueError(f'add_norm_quantize: w must be ({K},) {dt}, contiguous')
     if scale is None or scale.dtype != torch.float32 or scale.numel() != M or not scale.is_contiguous():
@@ -291,6 +293,15 @@ def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offs
                                               0 if xout is None else xout.stride(0), pq, p4, _ldq(q4), ps, M, K, stream())
         if rc:
             _lib.failed('tcq_add_norm_quantize', rc)
+
+
+def _apart(M, H, D, tok, head):
+    """Whether the rows of an output (M tokens of H heads of D values, these strides) are M * H different ones: no row is written twice."""
+    if M < 2:
+        return H < 2 or head >= D
+    if H < 2:
+        return tok >= D
+    return (head >= D and tok >= (H - 1) * head + D) or (tok >= D and head >= (M - 1) * tok + D)
 
 
 def _q4_holds(q4, M, K, what):
@@ -351,7 +362,7 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
     """Rotary positions with one or several axes (tcq_rope_axes) of q (M, Hq, D) and k (M, Hk, D) or None, BF16 / FP16 / FP32, any token
     and head strides (views into a q | k | v row). pos (A, M) or (M,) int32 / int64; freq (R / 2,) float64 and axis (R / 2,) int32 as
     rope_frequencies makes them, the R first values of a head turn. Outputs None: in place. adjacent: pairs (2 i, 2 i + 1) instead of
-    (i, i + R / 2). inverse: turns back, which is also the gradient."""
+    (i, i + R / 2). inverse: turns back, which is also the gradient. An output's rows may not overlap each other."""
     if q_out is None:
         q_out = q
     if k is None:
@@ -365,7 +376,7 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
     half, wide = freq.numel(), pos.dtype
     if not (len(size) == 3 and size == q_out.shape and q_out.dtype == dt in _ROPE_TYPES and sq[2] == so[2] == 1 and len(ps) == 2
             and ps[1] == size[0] and (wide == torch.int32 or wide == torch.int64) and freq.dtype == torch.float64 and 0 < 2 * half <= size[2]
-            and freq.is_contiguous()
+            and freq.is_contiguous() and _apart(size[0], size[1], size[2], so[0], so[1])
             and (axis is None or (axis.dtype == torch.int32 and axis.numel() == half and axis.is_contiguous()))):
         _rope_refuse(q, q_out, pos, freq, axis)
     M, Hq, D = size
@@ -378,6 +389,8 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
         if not (len(ks) == 3 and ks == ko.shape and ks[0] == M and ks[2] == D and k.dtype == ko.dtype == dt and sk[2] == sko[2] == 1):
             raise ValueError(f'rope_axes: k and its output must be ({M}, heads, {D}) {dt} with contiguous values')
         Hk = ks[1]
+        if not _apart(M, Hk, D, sko[0], sko[1]):
+            raise ValueError(_ROPE_OVERLAP)
     pq, pk, pp, pf, pa, pqo, pko = _ptrs('rope_axes', q, k, pos, freq, axis, q_out, ko)
     if M:
         rc = _lib.lib().tcq_rope_axes(pq, sq[0], sq[1], pqo, so[0], so[1], Hq, pk, sk[0], sk[1], pko, sko[0], sko[1], Hk, DTYPE[dt], pp,
@@ -388,6 +401,7 @@ def rope_axes(q, k, pos, freq, axis=None, q_out=None, k_out=None, adjacent=False
 
 
 _ROPE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_ROPE_OVERLAP = 'rope_axes: rows of an output (in place: of the input) overlap; an expanded tensor needs an output of its own'
 
 
 def _rope_refuse(q, q_out, pos, freq, axis):
@@ -397,6 +411,8 @@ def _rope_refuse(q, q_out, pos, freq, axis):
     _heads(q_out, 'rope_axes q_out', q.shape[2])
     if q_out.shape != q.shape or q_out.dtype != q.dtype:
         raise ValueError('rope_axes: q and its output must have the same size and type')
+    if not _apart(*q.shape, *q_out.stride()[:2]):
+        raise ValueError(_ROPE_OVERLAP)
     if pos.dim() not in (1, 2) or pos.shape[-1] != q.shape[0] or pos.dtype not in (torch.int32, torch.int64):
         raise ValueError(f'rope_axes: pos must be (axes, {q.shape[0]}) int32 or int64, got {tuple(pos.shape)} {pos.dtype}')
     raise ValueError(f'rope_axes: freq must be contiguous float64 of at most {q.shape[2] // 2} pairs and axis int32 of as many')
