@@ -53,3 +53,16 @@ def test_outputs_whose_rows_overlap_are_refused():
             K.add_norm_quantize(t, t, w, 1e-6, codes, s, x)
     with pytest.raises(_lib.TcqError):
         K.add_norm_quantize(x[:1], x[:1], w, 1e-6, codes[:1], s[:1], torch.zeros(1, D).expand(1, D))
+
+
+def test_frequencies_of_no_whole_pairs_or_other_sections_are_refused():
+    for R in (65, 1, 0, -2):
+        with pytest.raises(ValueError):
+            K.rope_frequencies(R)
+    for sections in ((10, 27, 27), (1, 2, 29), (0, 32)):              # interleaved, an axis would come out with other than its pairs
+        with pytest.raises(ValueError):
+            K.rope_frequencies(2 * sum(sections), sections=sections, interleaved=True)
+        assert K.rope_frequencies(2 * sum(sections), sections=sections)[1].bincount(minlength=3).tolist()[:len(sections)] == list(sections)
+    for sections in ((24, 20, 20), (32, 32), (3, 3, 2), (22, 21, 21), (8,)):
+        axis = K.rope_frequencies(2 * sum(sections), sections=sections, interleaved=True)[1]
+        assert [int((axis == a).sum()) for a in range(len(sections))] == list(sections)

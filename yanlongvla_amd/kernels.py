@@ -336,16 +336,20 @@ def _ptrs(what, *ts):
 def rope_frequencies(R, theta=10000.0, sections=None, interleaved=False, device=None):
     """(freq, axis) of rope_axes for R rotated values of a head: freq[i] = theta^(-2 i / R) (float64), and the axis of every pair:
     sections (pairs per axis, R / 2 in all) one after the other, or interleaved (axis i % A for as long as the axis has pairs left, the
-    first axis after that); None: one axis."""
+    first axis after that: sections that do not come out so are refused); None: one axis."""
+    if R < 2 or R % 2:
+        raise ValueError(f'rope_frequencies: {R} values are no whole pairs')
     half = R // 2
     freq = torch.tensor([float(theta) ** (-i / half) for i in range(half)], dtype=torch.float64, device=device)
     if sections is None:
         return freq, torch.zeros(half, dtype=torch.int32, device=device)
-    if sum(sections) != half or R % 2:
+    if sum(sections) != half:
         raise ValueError(f'rope_frequencies: the sections {tuple(sections)} must add up to {half} pairs')
     A = len(sections)
     if interleaved:
         axis = [i % A if i // A < sections[i % A] else 0 for i in range(half)]
+        if any(axis.count(a) != n for a, n in enumerate(sections)):
+            raise ValueError(f'rope_frequencies: the sections {tuple(sections)} do not interleave (an axis has more pairs than its turns)')
     else:
         axis = [a for a, n in enumerate(sections) for _ in range(n)]
     return freq, torch.tensor(axis, dtype=torch.int32, device=device)
