@@ -250,8 +250,10 @@ int tcq_post_add_norm_pre(const void* acc, int acc_dtype, int lda, int col0, con
  * gives tcq_gemm_i8): h = x + r rounded to dtype (r NULL: h = x), n = h / sqrt(mean(h^2) + eps) * (offset + w) (offset 1: Gemma's weights,
  * 0: plain ones), scale[t] = max|n| / 127 (1 for a row of zeros), q = rint(n / scale). x, r, xout (M, K) of dtype F32, BF16 or F16 with row
  * strides in elements, w (K,) of dtype; xout (NULL: not stored) may be x or r; q (M, K) int8 contiguous and / or q4 / ldq as tcq_pre.
- * FP32 sums; n itself is not rounded before its codes. A row with a value that is not finite has scale NaN. K <= 32768. No
- * reference counterpart: the reference leaves the policy's norms to PyTorch. */
+ * FP32 sums; n itself is not rounded before its codes. A row with a value that is not finite has scale NaN; a finite row whose sum of squares
+ * is past FP32 (values of about 1e19 and more) has norm 0 like in any FP32 RMSNorm, so scale 1 and codes 0; without an eps the
+ * squares may not fall below FP32 either (values of about 1e-19). K <= 32768. No reference counterpart: the reference leaves the policy's
+ * norms to PyTorch. */
 int tcq_add_norm_quantize(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, float eps, float offset, int dtype, void* xout,
                           int64_t ldo, int8_t* q, int32_t* q4, int ldq, float* scale, int M, int K, tcq_stream_t stream);
 
@@ -304,7 +306,7 @@ size_t tcq_attend_static_floats(void);
  * tensor only), D values each: pair i of the first R of a head's values turns by a = pos[axis[i]] * freq[i], (x1, x2) ->
  * (x1 cos a - x2 sin a, x2 cos a + x1 sin a), or by -a with inverse != 0 (the gradient of the rotation, and the way back). The pairs
  * are (i, i + R / 2), or (2 i, 2 i + 1) with adjacent != 0; the values from R on are copied. x, out: dtype F32, BF16 or F16, token and
- * head strides in elements, a head's values contiguous; out may be x (in place). pos: A x M int32 (pos64 = 0) or int64, strides in
+ * head strides in elements, a head's values contiguous; out may be x (in place), its rows may not overlap each other. pos: A x M int32 (pos64 = 0) or int64, strides in
  * elements; freq (R / 2,) FP64, radians per position; axis (R / 2,) int32 (NULL: all 0; outside 0 .. A - 1: the pair is not turned).
  * Angles are reduced in FP64. No reference counterpart: the reference leaves positions to PyTorch. */
 int tcq_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head, int Hq, const void* k,
@@ -338,13 +340,15 @@ int tcq_kv8_read(const int8_t* k8, const int8_t* v8, const float* scale, const i
                  int nblk, void* k, void* v, int dtype, tcq_stream_t stream);
 /* Attention over the cache: o = softmax(score_scale q k^T) v, query head i over KV head i / (Hq / Hk), sequence b's rows cu[b] ..
  * cu[b + 1] - 1 (cu NULL: most rows each) of q (rows, Hq, D; BF16 or F16, 16-byte aligned, strides in elements, multiples of 8) over its
- * first lens[b] positions; with causal, row i of n sees positions j <= lens[b] - n + i. o (rows, Hq, D) contiguous, of q's type. A row
+ * first lens[b] positions (those that the cache holds, where lens[b] is past its capacity); with causal, row i of n sees positions
+ * j <= lens[b] - n + i. o (rows, Hq, D) contiguous, of q's type. A row
  * that sees nothing is zeros; another query row with a value that is not finite is NaN; rows of no sequence are left as they were. keys:
  * about the most positions that a sequence has (it sets how far the work is split, never the result's meaning). part: workspace of
  * tcq_kv8_attend_floats(...) floats, 16-byte aligned (NULL where that is 0), not shared by calls that overlap. Scores from the query as
  * 16-bit integers (within 2^-16 of the row's largest value) and the probabilities as 16-bit integers of their block's maximum, exact
- * int32 products with the codes, FP32 maximum, sum and outputs (many rows of D up to 128: FP16 probabilities of the running maximum
- * instead). */
+ * int32 products with the codes, FP32 maximum, sum and outputs. Calls of D up to 128 with at least 512 groups of 32 rows (a KV head's query
+ * rows and heads of one sequence; a sequence's last group may be short): FP16 probabilities of the running maximum instead, 2.6e-4 against
+ * 2.4e-4 of the result (FP16's rounding alone 2.1e-4). The sum is always one of the rounded probabilities. Scores up to 2^26 in magnitude. */
 int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, const int32_t* lens, int rows, int most, int B,
                    int Hq, int Hk, int D, int nblk, const int8_t* k8, const int8_t* v8, const float* scale, int causal, float score_scale,
                    int keys, float* part, void* o, tcq_stream_t stream);

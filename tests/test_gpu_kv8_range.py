@@ -78,13 +78,13 @@ FORMS = [(2, 16, 8, 1, 256, 300), (2, 16, 8, 1, 256, 3000), (1, 40, 4, 2, 64, 15
 
 
 @pytest.mark.parametrize('dt', [BF, HF])
-@pytest.mark.parametrize('logit', [100.0, 400.0, 700.0, 1500.0, 5000.0, 1e5])
+@pytest.mark.parametrize('logit', [100.0, 400.0, 700.0, 1500.0, 5000.0, 1e5, 1e7])
 @pytest.mark.parametrize('B,M,Hq,Hk,D,n', FORMS)
 def test_large_scores_pick_their_key(B, M, Hq, Hk, D, n, logit, dt):
     """Every query row is a multiple of one key, whose score is `logit`, several standard deviations above the others': the
     output is that key's value."""
     from yanlongvla_amd import kernels as K
-    logit = min(logit, 1e5 if dt == BF else 1e4)                       # (FP16 queries end at 65504)
+    logit = min(logit, 1e7 if dt == BF else 1e4)                       # (FP16 queries end at 65504)
     cache = fill(B, n, Hk, D, dt, seed=11)
     k, v = held(cache, n)
     pick = torch.randint(0, n, (B, M, Hq), generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)

@@ -163,7 +163,7 @@ __device__ __forceinline__ u32 kv_pair(float x, float y, int dt) {   // (finite 
 }
 
 // grid (2 x D / 64 x blocks a window may touch, H, B): 256 pieces of 16 values of a block's keys (even block index) or values; k, v (B, n, H, D),
-// row i of sequence b is position first[b] + i, zeros from lens[b] on. MI355X: 6 x 1024 rows, 8 heads of 128 11.6 us (38 MB, 3.2 TB/s).
+// row i of sequence b is position first[b] + i, zeros from lens[b] on. MI355X: 6 x 1024 rows, 8 heads of 128 11.2 us (38 MB, 3.4 TB/s).
 template <int D>
 __global__ __launch_bounds__(KT) void k_kv8_read(KvRead a) {
     const int b = blockIdx.z, h = blockIdx.y, bx = blockIdx.x / (D / 64), val = bx & 1, u = blockIdx.x % (D / 64) * KT + threadIdx.x;
@@ -289,12 +289,15 @@ __device__ __forceinline__ void widen(uint4_t w, half8_t& a, half8_t& b) {
 // A wave holds one block's keys or values at a time and leaves the overlap of loads, matrix and vector instructions to the other waves of
 // its SIMD (four of them for D up to 128): one wave issues a vector instruction every 7 to 13 cycles here, four together every 3 to 5. With
 // the next block's keys and values already under way (twice the registers, half the waves) 968 causal rows of 16 x 128 took 19.5 us instead
-// of 16.6, 4096 rows 140 instead of 131. D = 256 in four waves, where two a SIMD are all that fit, does fetch the next keys: 131000 keys of
-// two sequences 25.5 us instead of 27.5 (4.6 TB/s; 16 sequences of 8 heads x 128 behind 8192 keys 40.8 us, 5.0 TB/s).
+// of 16.6, 4096 rows 140 instead of 131 (both before the grid below). D = 256 in four waves, where two a SIMD are all that fit, does fetch
+// the next keys: 131000 keys of two sequences 25.3 us instead of 27.5 (4.6 TB/s; 16 sequences of 8 heads x 128 behind 4 to 8 thousand keys
+// 40.3 us, 5.1 TB/s).
+// Range: scores of up to 2^26 (FP32 tells those past 2^23 apart by whole numbers only). RT = 1 holds the outputs in FP32 as they are, so values
+// from about 1e-35 to 1e35 keep their digits; RT > 1 in units of the row's own.
 // Grid (Hk x parts, B, row tiles): workgroups go to the eight XCDs in turn, so with eight KV heads an XCD's L2 sees one head's keys, and a
 // tile's workgroups of all sequences come before the next tile's, the last tiles first, as they see the most keys. With the tiles of a head
-// side by side and the first ones first: 968 causal rows of 16 x 128 16.7 us against 13.2, of 8 x 256 16.8 against 14.6, 4096 rows 129
-// against 113, 90 rows behind 1936 keys, 8 sequences of 16 x 64 23.4 against 17 (2 x 1024 rows behind 4096 keys 103 against 104).
+// side by side and the first ones first: 968 causal rows of 16 x 128 15.3 us against 11.7, of 8 x 256 15.3 against 12.9, 4096 rows 117
+// against 96, 90 rows behind 1846 keys, 8 sequences of 16 x 64 31.3 against 16.7 (2 x 1024 rows behind up to 4096 keys 92.6 against 93.4).
 template <int D, int W, int RT>
 __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_attend(KvAttend a) {
     constexpr int KS = D / 64, DTL = D / 16;
@@ -646,7 +649,7 @@ __global__ __launch_bounds__(W * 64, D == 256 || RT == 2 ? 2 : 4) void k_kv8_att
 }
 
 // The splits' outputs of a row joined, weights exp2(m_s - max m). Few splits (at most 8): D / 4 threads a row, 4 dims each, every load at entry.
-// A launch and two memory latencies: 256 rows x 8 parts x 128 4.5 us.
+// A launch and two memory latencies: 256 rows x 8 parts x 128 4.8 us.
 template <int D>
 __global__ __launch_bounds__(KT) void k_kv8_join_few(KvAttend a) {
     constexpr int TD = D / 4, MS = 8;
@@ -747,14 +750,17 @@ bool kv_size(int B, int H, int nblk) { return B > 65535 || H > 65535 || nblk > (
 
 // How a call is split: the waves W of a workgroup, which take the blocks of 16 RT rows of a KV head in turn, and the parts S of their keys.
 //   Two tiles of 16 rows a wave (D up to 128; 256 has no registers left for it) where that still makes two workgroups a CU: 2 x 1024 rows of
-//   16 heads x 128 behind 4096 keys 104 us against 115, 4096 rows 112 against 125, 4 x 1024 rows of 16 heads x 64 28 against 32; with half
-//   as many workgroups it loses (968 rows of 16 x 128 14.5 against 13.2), three or four tiles gain nothing (D = 64: 31).
-//   Few rows over up to 16 blocks: one launch of eight waves (50 rows of 4 sequences behind 800 keys, D = 256: 10.8 us against 12.8 in parts
-//   of four waves with their join, 10 rows of 16 sequences 10.6 against 13.8; one row behind 968 10.0 against 9.0, but a call from Python
-//   12 against 16).
-//   Else four waves (968 causal rows of 8 heads x 256 14.5 us, with eight 18.4), in as many parts as give every CU a workgroup. Where that is
+//   16 heads x 128 behind up to 4096 keys 93.5 us against 100.6, 4096 rows 95.8 against 106.2, 4 x 1024 rows of 16 heads x 64 25.7 against
+//   28.9; with half as many workgroups it loses (968 rows of 16 x 128 13.8 against 12.7). Single rows of as many sequences go there too, by
+//   the same rule, and are bound by memory either way: 64 sequences of 8 heads x 128 behind 4096 keys 96 against 99.5 (5.6 TB/s), 128 behind
+//   1 to 2 thousand 76 against 74.
+//   Few rows over up to 16 blocks: one launch of eight waves (50 rows of 4 sequences behind 800 keys, D = 256: 10.3 us against 12.6 in parts
+//   of four waves with their join, 10 rows of 16 sequences 10.4 against 13.7; one row behind 968 9.9 against 8.9, but a call from Python
+//   12 against 15.5).
+//   Else four waves (968 causal rows of 8 heads x 256 13.5 us, with eight 17.0), in as many parts as give every CU a workgroup. Where that is
 //   fewer than 4 and the parts stay long, as many as fit: the lengths of a batch differ (16 sequences of 4 to 8 thousand keys, 8 heads of
-//   128: 47 us against 58).
+//   128: 44.3 us against 55.5).
+//   (Times of calls one after the other in a captured graph, joins included.)
 struct KvPlan {
     int W, S, RT;
 };

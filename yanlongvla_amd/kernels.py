@@ -270,7 +270,8 @@ def post_add_norm_pre(acc, s, rs, sv, bias, x, xout, w=None, eps=0.0, su=None, q
 def add_norm_quantize(x, r, w, eps, q=None, scale=None, xout=None, q4=None, offset=1.0):
     """h = x + r (r None: x), rounded to x's type and stored in xout where that is given (it may be x or r), then INT8 rows of
     RMSNorm(h) * (offset + w): q (M, K) int8 and / or q4 (as in pre), scale (M,) FP32, what gemm_i8 takes. x, r, xout (M, K) BF16 / FP16
-    / FP32 with contiguous rows of any stride (xout's may not overlap), w (K,) of that type; offset 1: Gemma's weights, 0: plain ones."""
+    / FP32 with contiguous rows of any stride (xout's may not overlap), w (K,) of that type; offset 1: Gemma's weights, 0: plain ones.
+    Scale 1 and codes 0: a row of zeros, or one whose sum of squares is past FP32 (values of about 1e19); scale NaN: a value not finite."""
     size, dt = x.shape, x.dtype
     M, K = size
     if dt not in DTYPE or dt not in (torch.bfloat16, torch.float16, torch.float32):
@@ -513,7 +514,8 @@ def kv8_read(cache, first, lens, n, dtype=None):
 def kv8_attend(q, cache, lens, o=None, causal=True, cu=None, most=None, scale=None, keys=None):
     """Attention of q (rows, Hq, D; BF16 / FP16, 16-byte aligned, token and head strides multiples of 8) over the first lens[b] rows (int32,
     on the device) of every sequence of the cache, Hq a multiple of its heads: o (rows, Hq, D). B equal shares of the rows, or cu and most
-    as in kv8_append. With causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended).
+    as in kv8_append. With causal, row i of a sequence's n sees positions up to lens[b] - n + i (its own, once it has been appended), and
+    with lens[b] past the capacity those of them that the cache holds.
     scale: of the scores, 1 / sqrt(D) by default; keys: about the longest length (the capacity by default), for the split of the work
     alone. A row that sees nothing is zeros; rows of no sequence (and a sequence's past `most`) are left as they were in o, and hold
     anything in a new one."""
