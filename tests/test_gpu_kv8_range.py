@@ -228,3 +228,14 @@ def test_huge_queries_of_tiny_keys(B, M, Hq, Hk, D, n, qe, ke):
     big = cache._replace(scale=scale)
     q = (rand(B * M, Hq, D, seed=62) * 2 * qe).to(BF)
     close(K.kv8_attend(q, big, ints([n] * B), causal=False), reference(q, *held(big, n), [n] * B, Hq // Hk))
+
+
+@pytest.mark.parametrize('B,M,Hq,Hk,D,n', FORMS)
+@pytest.mark.parametrize('causal', [False, True])
+def test_a_score_scale_of_zero_gives_means(B, M, Hq, Hk, D, n, causal):
+    from yanlongvla_amd import kernels as K
+    cache = fill(B, n, Hk, D, seed=71)
+    q = rand(B * M, Hq, D, seed=72, dt=BF)
+    zero = reference(q * 0, *held(cache, n), [n] * B, Hq // Hk, causal)
+    close(K.kv8_attend(q, cache, ints([n] * B), causal=causal, scale=0.0), zero)
+    close(K.kv8_attend(q * 0, cache, ints([n] * B), causal=causal), zero)
