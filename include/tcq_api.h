@@ -348,7 +348,8 @@ int tcq_kv8_read(const int8_t* k8, const int8_t* v8, const float* scale, const i
  * 16-bit integers (within 2^-16 of the row's largest value) and the probabilities as 16-bit integers of their block's maximum, exact
  * int32 products with the codes, FP32 maximum, sum and outputs. Calls of D up to 128 with at least 512 groups of 32 rows (a KV head's query
  * rows and heads of one sequence; a sequence's last group may be short): FP16 probabilities of the running maximum instead, 2.6e-4 against
- * 2.4e-4 of the result (FP16's rounding alone 2.1e-4). The sum is always one of the rounded probabilities. Scores up to 2^26 in magnitude. */
+ * 2.4e-4 of the result (FP16's rounding alone 2.1e-4). The sum is always one of the rounded probabilities. Scores up to 2^26 in
+ * magnitude; values of 1e-35 to 1e35 (below, digits get lost in FP32: 3 % at 1e-37; the calls with FP16 probabilities keep them). */
 int tcq_kv8_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, const int32_t* lens, int rows, int most, int B,
                    int Hq, int Hk, int D, int nblk, const int8_t* k8, const int8_t* v8, const float* scale, int causal, float score_scale,
                    int keys, float* part, void* o, tcq_stream_t stream);
