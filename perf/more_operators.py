@@ -223,7 +223,7 @@ def run(st):
             kernels.paged_append(pool, st['k'], st['v'], st['table'], st['lens'], st['start'], cu=st['cu'], most=st['most'])
             return dict(k=st['pk'], v=st['pv'])
         st['flat'].copy_(st['saved'])
-        book = kernels.PageTable(st['table'], st['lens'], st['refs'], st['free'], st['lack'])
+        book = kernels.PageTable(st['table'], st['lens'], st['refs'], st['free'], st['lack'], case['T'])
         if kind == 'compact':
             kernels.pages_compact(book, pool)
             return dict(table=st['table'], refs=st['refs'], k=st['pk'], v=st['pv'])
