@@ -588,6 +588,58 @@ int tcq_gemmf_w8_hT(const int8_t* W, const void* hT, int ldh, const float* rs, f
 int tcq_gemmf_tcq_hT(const void* bits, const int8_t* t8, const void* hT, int ldh, const float* rs, float* z, int M, int N, int K,
                      int nb0, int nb1, tcq_stream_t stream);
 
+/* A cache of 16-bit key / value rows in pages that sequences share (beyond the reference's helpers). A layer's pool: keys and values (pages, heads,
+ * page_rows, D) each, page_rows a power of two from 16 on. The bookkeeping, one for all layers of a model, lives on the device: table (B, per_seq),
+ * the pages of each sequence in order and -1 behind them; lens (B), the rows that it holds, in ceil(lens / page_rows) pages; refs (pages), the sequences
+ * that hold a page; free, bit p % 32 of word p / 32 set where refs[p] is 0; lack, what calls could not do. At most 4096 sequences.
+ * Graph-capturable; what a call does follows from its inputs alone (pages are taken from the lowest free one on, for the sequences in order). All
+ * calls on one bookkeeping belong on one stream, or on streams that wait for each other.
+ *
+ * tcq_pages_take: room for take[b] >= 0 more rows of every sequence: start[b] = lens[b], lens[b] += take[b]. A last page that is partly filled
+ *   and held by other sequences too is replaced by a copy (k, v: the pools of all layers, (layers, pages) pages of page_bytes, a multiple of 16), if rows
+ *   are taken; one that loses its last sequence so is free after the call. A sequence that lacks pages (those before it are served first) or entries
+ *   stays as it is and adds one to lack. moves: 2 B + 1 ints of workspace.
+ * tcq_pages_fork: sequence dst[i], which must hold nothing, comes to hold the rows of src[i], in the same pages. A pair that names no sequence, a dst
+ *   that holds rows or that an earlier pair names, or a src that is a dst of the call, is left out and adds one to lack.
+ * tcq_pages_trim: sequence b keeps its first keep[b] rows; pages behind them that no other sequence holds are free.
+ * tcq_pages_compact: the pages in use become the lowest ones, U in all: the i-th used page from U on moves (in all layers) to the i-th free one below U.
+ *   moves: 2 pages + 2 ints of workspace.
+ * tcq_pages_copy: page src[i] to page dst[i] in all layers, n pairs; pairs outside the pool are left out, no page may be a dst twice, or a dst and a
+ *   src. The bookkeeping is not told.
+ * tcq_paged_append: rows k, v (any strides in elements) to positions start[b] + i of their sequence: B equal shares of `most` rows, or rows cu[b] ..
+ *   cu[b + 1] - 1, at most `most` of them. Rows at or past lens[b], and those whose entry names no page, are dropped. */
+int tcq_pages_take(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows,
+                   const int32_t* take, int32_t* start, void* k, void* v, int layers, int64_t page_bytes, int32_t* moves, tcq_stream_t stream);
+int tcq_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows,
+                   const int32_t* src, const int32_t* dst, int n, tcq_stream_t stream);
+int tcq_pages_trim(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows,
+                   const int32_t* keep, tcq_stream_t stream);
+int tcq_pages_compact(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows, void* k,
+                      void* v, int layers, int64_t page_bytes, int32_t* moves, tcq_stream_t stream);
+int tcq_pages_copy(void* k, void* v, int layers, int pages, int64_t page_bytes, const int32_t* src, const int32_t* dst, int n, tcq_stream_t stream);
+int tcq_paged_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, const int32_t* cu, int rows, int most,
+                     int B, int H, int D, void* pk, int64_t k_page, int64_t pk_head, int64_t pk_tok, void* pv, int64_t v_page, int64_t pv_head,
+                     int64_t pv_tok, int pages, int page_rows, const int32_t* table, int per_seq, const int32_t* lens, const int32_t* start,
+                     tcq_stream_t stream);
+
+/* Softmax attention of q (rows, Hq, D), BF16 or FP16, D a multiple of 8 up to 256, over the first lens[b] rows of every sequence of such a cache (Hk
+ * heads, Hq a multiple of Hk; q, k, v of one type; strides in elements, multiples of 8; 16-byte aligned): o (rows, Hq, D), contiguous. Rows of
+ * sequence b: B equal shares of `most` rows, or rows cu[b] .. cu[b + 1] - 1, at most `most` of them. causal: row i of a sequence's n sees
+ * positions up to lens[b] - n + i. A row that sees nothing is zeros; rows of no sequence are left as they are. An entry of the table outside the
+ * pool counts as page 0. keys: about the longest length, for the split of the work alone. part: tcq_paged_attend_floats(...) floats of workspace
+ * (0: none), 16-byte aligned, of this call alone. */
+int64_t tcq_paged_attend_floats(int rows, int most, int B, int Hq, int Hk, int D, int keys);
+int tcq_paged_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, const int32_t* lens, int rows, int most, int B, int Hq,
+                     int Hk, int D, const void* k, int64_t k_page, int64_t k_head, int64_t k_tok, const void* v, int64_t v_page, int64_t v_head,
+                     int64_t v_tok, int pages, int page_rows, const int32_t* table, int per_seq, int causal, float score_scale, int keys, float* part,
+                     void* o, tcq_stream_t stream);
+/* The same of query rows that all see the keys of their sequence in a batch of an encoder's states, k and v of `keys` rows a sequence: the first lens[b]
+ * (NULL: all) of those with mask[b, j] not 0 (NULL: all; mask_seq apart). Workspace: tcq_cross_attend_floats of the same sizes. */
+int64_t tcq_cross_attend_floats(int rows, int most, int B, int Hq, int Hk, int D, int keys);
+int tcq_cross_attend(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, int rows, int most, int B, int Hq, int Hk, int D,
+                     const void* k, int64_t k_seq, int64_t k_head, int64_t k_tok, const void* v, int64_t v_seq, int64_t v_head, int64_t v_tok, int keys,
+                     const int32_t* lens, const uint8_t* mask, int64_t mask_seq, float score_scale, float* part, void* o, tcq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,8 +90,19 @@ SIGNATURES = {
     'tcq_kv8_read': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P],
     'tcq_kv8_attend': [_P, _L, _L, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _I, _F, _I, _P, _P, _P],
     'tcq_kv8_attend_floats': [_I, _I, _I, _I, _I, _I, _I],
+    'tcq_pages_take': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _L, _P, _P],
+    'tcq_pages_fork': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P],
+    'tcq_pages_trim': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
+    'tcq_pages_compact': [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _L, _P, _P],
+    'tcq_pages_copy': [_P, _P, _I, _I, _L, _P, _P, _I, _P],
+    'tcq_paged_append': [_P, _L, _L, _P, _L, _L, _P, _I, _I, _I, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _P, _I, _P, _P, _P],
+    'tcq_paged_attend_floats': [_I, _I, _I, _I, _I, _I, _I],
+    'tcq_paged_attend': [_P, _L, _L, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _P, _I, _I, _F, _I, _P, _P, _P],
+    'tcq_cross_attend_floats': [_I, _I, _I, _I, _I, _I, _I],
+    'tcq_cross_attend': [_P, _L, _L, _I, _P, _I, _I, _I, _I, _I, _I, _P, _L, _L, _L, _P, _L, _L, _L, _I, _P, _P, _L, _F, _P, _P, _P],
 }
-_RESTYPE = {'tcq_version': ctypes.c_char_p, 'tcq_repack_words': _L, 'tcq_kv8_attend_floats': _L, 'tcq_attend_static_floats': ctypes.c_size_t}
+_RESTYPE = {'tcq_version': ctypes.c_char_p, 'tcq_repack_words': _L, 'tcq_kv8_attend_floats': _L, 'tcq_paged_attend_floats': _L,
+            'tcq_cross_attend_floats': _L, 'tcq_attend_static_floats': ctypes.c_size_t}
 
 MAX_SEGS = 4
 

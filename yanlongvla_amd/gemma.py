@@ -78,7 +78,7 @@ class GemmaAttention(nn.Module):
         """Attention of the projected q / k / v (the cache rows, if any, before this call's own keys / values). Device
         BF16 tensors go to the HIP attention kernel; host tensors (CPU twins in tests) to the same formula in PyTorch. cache_k may
         be a kernels.KV8Rows: the rows (at most 64) then go into that 8-bit cache (causal_offset: its length, or None for every row to see
-        all)."""
+        all), or a kernels.PagedRows: equal shares of the rows go to the sequences of its table."""
         if hasattr(cache_k, 'core'):
             return cache_k.core(q, k, v, self.heads, causal_offset is not None)
         if self._device(q):
@@ -209,6 +209,78 @@ class KV8Cache:
         self.end.add_(1)
 
 
+class PagedKVCache:
+    """The key / value rows of a batch of sequences in pages of one pool (kernels.kv_pages, page_table), which they share: prompts that begin alike
+    (fork), candidates that are tried and given up (trim, free). A decode step takes one row of every active sequence (x (sequences, width) in
+    BackbonePolicy.decode_step_cached) and makes their room itself, on the device: a captured step can be replayed. Rows that the pool has no
+    page for are dropped and counted in table.lack."""
+
+    def __init__(self, layers, sequences, pages, D, device, rows=64, per_sequence=None, heads=1, dtype=torch.bfloat16):
+        from . import kernels
+        self.sequences = sequences
+        self.pool = kernels.kv_pages(pages, heads, D, device, rows, dtype, layers)
+        self.table = kernels.page_table(sequences, per_sequence or pages, pages, device, rows)
+        self.layers = [kernels.Pages(k, v) for k, v in zip(*self.pool)]
+        self.active = torch.ones(sequences, dtype=torch.int32, device=device)         # rows of each sequence that a decode step takes
+        self.start = torch.zeros(sequences, dtype=torch.int32, device=device)
+
+    def _only(self, sequence, n):
+        """take and cu of n rows of one sequence and none of the others."""
+        take = torch.zeros_like(self.active)
+        take[sequence:sequence + 1].fill_(n)
+        cu = torch.zeros(self.sequences + 1, dtype=torch.int32, device=take.device)
+        cu[sequence + 1:].fill_(n)
+        return take, cu
+
+    def extend(self, ks, vs, sequence):
+        """Rows ks[i], vs[i] (n, heads * D) of every layer i behind those of one sequence, as a prefill returns them."""
+        from . import kernels
+        n, D = ks[0].shape[0], self.pool.k.shape[-1]
+        take, cu = self._only(sequence, n)
+        start = kernels.pages_take(self.table, self.pool, take)
+        for layer, k, v in zip(self.layers, ks, vs):
+            kernels.paged_append(layer, k.reshape(n, -1, D), v.reshape(n, -1, D), self.table.table, self.table.lens, start, cu, n)
+
+    def chunk(self, sequence, n):
+        """Room for n more rows of one sequence: the PagedRows of every layer for the call that writes them and attends (BackbonePolicy.prefill_chunk)."""
+        from . import kernels
+        take, cu = self._only(sequence, n)
+        start = kernels.pages_take(self.table, self.pool, take)
+        return [kernels.PagedRows(layer, self.table.table, self.table.lens, start, cu=cu, most=n) for layer in self.layers]
+
+    def fork(self, src, dst):
+        """Sequences dst, which hold nothing, come to hold the rows of sequences src (int32 on the device, one each)."""
+        from . import kernels
+        kernels.pages_fork(self.table, src, dst)
+
+    def trim(self, keep):
+        """Every sequence keeps its first keep[b] rows (int32 on the device); 0 frees it."""
+        from . import kernels
+        kernels.pages_trim(self.table, keep)
+
+    def compact(self):
+        """The pages in use move to the lowest places of the pool."""
+        from . import kernels
+        kernels.pages_compact(self.table, self.pool)
+
+    def take(self, rows):
+        """Room for rows[b] more rows of every sequence: the PagedRows of every layer for calls that write and attend to them (the expert's denoising steps,
+        ExpertPolicy.set_prefix: action tokens of all sequences, replaced at each step)."""
+        from . import kernels
+        start = kernels.pages_take(self.table, self.pool, rows)
+        return [kernels.PagedRows(layer, self.table.table, self.table.lens, start) for layer in self.layers]
+
+    def rows(self, i):
+        """Layer i's pages as the layers take them: (kernels.PagedRows, None, None). The first layer's call makes the room of a step."""
+        from . import kernels
+        if i == 0:
+            kernels.pages_take(self.table, self.pool, self.active, self.start)
+        return kernels.PagedRows(self.layers[i], self.table.table, self.table.lens, self.start), None, None
+
+    def advance(self):
+        pass
+
+
 EXPERT = dict(layers=18, width=1024, hidden=4096, heads=8, head_dim=256, action_dim=32)
 BACKBONE = dict(layers=18, width=2048, hidden=16384, heads=8, head_dim=256, vocab=257152)
 
@@ -231,7 +303,8 @@ class ExpertPolicy(nn.Module):
 
     def set_prefix(self, ks, vs):
         """Per-layer prefix keys / values (T, head_dim), as the backbone's prefill leaves them; or, with vs all None, a kernels.KV8Rows
-        per layer whose start is the prefix's length (the action tokens of a step, at most 64, replace those of the step before)."""
+        per layer whose start is the prefix's length (the action tokens of a step, at most 64, replace those of the step before), or a
+        kernels.PagedRows per layer (PagedKVCache.take: the action tokens of several sequences, one after the other)."""
         self.prefix_k, self.prefix_v = list(ks), list(vs)
 
     def velocity(self, x_t):
@@ -277,9 +350,17 @@ class BackbonePolicy(nn.Module):
             vs.append(v)
         return self.stack.norm(h), ks, vs
 
+    def prefill_chunk(self, x, cache, sequence):
+        """x (n, width), the next part of a sequence's prefix, behind the rows that a PagedKVCache holds of it: the hidden states, with the rows written
+        into the cache. Parts of any length give the rows of one prefill."""
+        h = x
+        for layer, rows in zip(self.stack.layers, cache.chunk(sequence, x.shape[0])):
+            h, _, _ = layer(h, rows, None, causal_offset=0)
+        return self.stack.norm(h)
+
     def decode_step_cached(self, x, cache):
         """decode_step on a KVCache: the same hidden state, with this token's keys / values written into the cache. On a KV8Cache: over
-        the rows that its 8 bits stand for."""
+        the rows that its 8 bits stand for. On a PagedKVCache: one row x (sequences, width) of every sequence."""
         from . import modules
         h = x
         with modules.deferred_outputs():                 # each layer's output goes straight to the next layer

@@ -565,6 +565,257 @@ class KV8Rows:
         return kv8_attend(q.reshape(M, heads, D), self.cache, lens, causal=causal, keys=self.keys).view(M, heads * D)
 
 
+# ------------------------------------------------------------------------------------- cache in pages, cross attention
+# A cache of 16-bit rows in pages that sequences share (include/tcq_api.h). Pages: one layer's keys and values (pages, H, T, D), or those of all
+# layers (layers, pages, H, T, D). PageTable: the bookkeeping of all layers, on the device: table (B, N), lens (B,), refs (pages,), free
+# ((pages + 31) / 32,) and lack (1,), int32; rows: T.
+Pages = collections.namedtuple('Pages', 'k v')
+PageTable = collections.namedtuple('PageTable', 'table lens refs free lack rows')
+PAGED_SEQUENCES = 4096
+
+
+def kv_pages(pages, H, D, device, rows=64, dtype=torch.bfloat16, layers=None):
+    """A pool of pages of `rows` key / value rows (a power of two from 16 on) of H KV heads of D values (a multiple of 8 up to 256); layers:
+    the pools of that many layers, whose page ids are the same (Pages(p.k[i], p.v[i]) is layer i's)."""
+    if rows < 16 or rows & (rows - 1) or D % 8 or not 8 <= D <= 256 or min(pages, H) < 1 or dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError('kv_pages: pages of 16, 32, 64, ... rows, head size a multiple of 8 up to 256, bfloat16 or float16, at least one page and head')
+    size = (() if layers is None else (layers,)) + (pages, H, rows, D)
+    return Pages(torch.zeros(size, dtype=dtype, device=device), torch.zeros(size, dtype=dtype, device=device))
+
+
+def page_table(B, N, pages, device, rows=64):
+    """The bookkeeping of B sequences (at most 4096) of up to N pages each, out of a pool of `pages` pages of `rows` rows, all free: its tensors
+    are views of one."""
+    if not (1 <= B <= PAGED_SEQUENCES and N >= 1 and pages >= 1) or rows < 16 or rows & (rows - 1):
+        raise ValueError(f'page_table: 1 to {PAGED_SEQUENCES} sequences, at least one page, of 16, 32, 64, ... rows')
+    words = (pages + 31) // 32
+    flat = torch.zeros(B * N + B + pages + words + 1, dtype=torch.int32, device=device)
+    table, lens, refs, free, lack = flat.split([B * N, B, pages, words, 1])
+    table.fill_(-1)
+    free.fill_(-1)
+    if pages % 32:
+        free[-1:].fill_((1 << pages % 32) - 1)
+    return PageTable(table.view(B, N), lens, refs, free, lack, rows)
+
+
+def _table(pt, what):
+    """Sizes (B, N, pages, rows of a page) of a bookkeeping whose tensors fit each other."""
+    table, lens, refs, free, lack, rows = pt
+    if len(table.shape) == 2 and len(refs.shape) == 1:
+        (B, N), P = table.shape, refs.shape[0]
+        if (lens.shape == (B,) and free.shape == ((P + 31) // 32,) and lack.shape == (1,) and 0 < B <= PAGED_SEQUENCES and N > 0 and P > 0
+                and table.dtype == lens.dtype == refs.dtype == free.dtype == lack.dtype == torch.int32
+                and table.is_contiguous() and lens.is_contiguous() and refs.is_contiguous() and free.is_contiguous()):
+            return B, N, P, rows
+    raise ValueError(f'{what}: these tensors are not those of a page_table')
+
+
+_PAGE_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _pool(pages, what, P, rows):
+    """(layers, bytes of a page) of a whole pool: contiguous, P pages of `rows` rows."""
+    k, v = pages
+    s = k.shape
+    if not (len(s) in (4, 5) and s == v.shape and s[-4] == P and s[-2] == rows and k.dtype == v.dtype and k.dtype in _PAGE_TYPES
+            and k.is_contiguous() and v.is_contiguous() and s[-1] % 8 == 0):
+        raise ValueError(f'{what}: k and v must be contiguous ([layers,] {P}, H, {rows}, D), bfloat16 or float16, as kv_pages makes them')
+    return s[0] if len(s) == 5 else 1, 2 * s[-3] * rows * s[-1]
+
+
+def pages_take(pt, pages, take, start=None):
+    """Room for take[b] (B, int32, on the device, 0: none) more rows of every sequence: returns start (B,), where they go, and raises pt.lens by
+    them. A last page that is partly filled and shared is copied in `pages` (the pools of all layers) first. A sequence that the free pages,
+    or its entries, do not suffice for (those before it come first) stays as it is and adds one to pt.lack; its rows are dropped by paged_append."""
+    size = _table(pt, 'pages_take')
+    pool = _pool(pages, 'pages_take', size[2], size[3])
+    B = size[0]
+    _counts('pages_take', take, B)
+    if start is None:
+        start = torch.empty_like(take)
+    else:
+        _counts('pages_take', start, B)
+    *book, tk, ts, pk, pv = _ptrs('pages_take', *pt[:5], take, start, *pages)
+    moves = torch.empty(2 * B + 1, dtype=torch.int32, device=take.device)
+    rc = _lib.lib().tcq_pages_take(*book, *size, tk, ts, pk, pv, *pool, moves.data_ptr(), stream())
+    if rc:
+        _lib.failed('tcq_pages_take', rc)
+    return start
+
+
+def pages_fork(pt, src, dst):
+    """Sequences dst (n,), which hold nothing, come to hold the rows of sequences src (n,), both int32 on the device, in the same pages. Pairs that
+    cannot be (see tcq_pages_fork) are left out and add one each to pt.lack."""
+    size, n = _table(pt, 'pages_fork'), src.numel()
+    _counts('pages_fork', src, n)
+    _counts('pages_fork', dst, n)
+    *book, ps, pd = _ptrs('pages_fork', *pt[:5], src, dst)
+    if n:
+        rc = _lib.lib().tcq_pages_fork(*book, *size, ps, pd, n, stream())
+        if rc:
+            _lib.failed('tcq_pages_fork', rc)
+
+
+def pages_trim(pt, keep):
+    """Every sequence keeps its first keep[b] rows (B, int32, on the device; more than it holds: all) and gives back the pages behind them: 0 frees it."""
+    size = _table(pt, 'pages_trim')
+    _counts('pages_trim', keep, size[0])
+    *book, pk = _ptrs('pages_trim', *pt[:5], keep)
+    rc = _lib.lib().tcq_pages_trim(*book, *size, pk, stream())
+    if rc:
+        _lib.failed('tcq_pages_trim', rc)
+
+
+def pages_compact(pt, pages):
+    """Moves the pages in use to the lowest places of the pool, in `pages` (the pools of all layers) and in the table: the pool's end is free then."""
+    size = _table(pt, 'pages_compact')
+    pool = _pool(pages, 'pages_compact', size[2], size[3])
+    *book, pk, pv = _ptrs('pages_compact', *pt[:5], *pages)
+    moves = torch.empty(2 * size[2] + 2, dtype=torch.int32, device=pt.table.device)
+    rc = _lib.lib().tcq_pages_compact(*book, *size, pk, pv, *pool, moves.data_ptr(), stream())
+    if rc:
+        _lib.failed('tcq_pages_compact', rc)
+
+
+def pages_copy(pages, src, dst):
+    """Page src[i] to page dst[i] (n,) int32 on the device, in all layers of `pages`: for pages that the caller keeps books of. Pairs outside the pool are left
+    out; no page may be a dst twice, or a dst and a src."""
+    shape = pages.k.shape
+    if len(shape) not in (4, 5):
+        raise ValueError('pages_copy: a pool as kv_pages makes it')
+    layers, size = _pool(pages, 'pages_copy', shape[-4], shape[-2])
+    n = src.numel()
+    _counts('pages_copy', src, n)
+    _counts('pages_copy', dst, n)
+    pk, pv, ps, pd = _ptrs('pages_copy', *pages, src, dst)
+    if n:
+        rc = _lib.lib().tcq_pages_copy(pk, pv, layers, shape[-4], size, ps, pd, n, stream())
+        if rc:
+            _lib.failed('tcq_pages_copy', rc)
+
+
+def _one_layer(pages, what):
+    """Sizes (pages, H, rows of a page, D) and strides of one layer's keys and values."""
+    k, v = pages
+    s, sk, sv = k.shape, k.stride(), v.stride()
+    if not (len(s) == 4 and s == v.shape and k.dtype == v.dtype and sk[3] == sv[3] == 1 and s[0] > 0 and s[2] >= 16 and s[2] & (s[2] - 1) == 0):
+        raise ValueError(f'{what}: k and v must be one layer\'s (pages, H, rows of a page, D) with contiguous values, pages of 16, 32, 64, ... rows')
+    return s, sk, sv, k.dtype
+
+
+def _tables(what, table, lens):
+    if not (len(table.shape) == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.shape[0] > 0 and table.shape[1] > 0):
+        raise ValueError(f'{what}: table must be a contiguous int32 (sequences, pages of one)')
+    _counts(what, lens, table.shape[0])
+    return table.shape
+
+
+def paged_append(pages, k, v, table, lens, start, cu=None, most=None):
+    """Writes rows k, v (rows, H, D; the pages' type, any token and head strides) to positions start[b] .. of their sequence in the pages (one layer's) that
+    table (B, N) names, all int32 on the device: B equal shares of the rows, or rows cu[b] .. cu[b + 1] - 1 (most: at least the rows
+    of any sequence). Rows at or past lens[b], the length with them, are dropped. What pages_take returns is start."""
+    ps, pk, pv, dt = _one_layer(pages, 'paged_append')
+    size, sk, sv = k.shape, k.stride(), v.stride()
+    if not (len(size) == 3 and size == v.shape and size[1] == ps[1] and size[2] == ps[3] and sk[2] == sv[2] == 1 and k.dtype == v.dtype == dt
+            and dt in _PAGE_TYPES):
+        raise ValueError(f'paged_append: k and v must be (rows, {ps[1]}, {ps[3]}) {dt} (bfloat16 or float16) with contiguous values')
+    B, N = _tables('paged_append', table, lens)
+    _counts('paged_append', start, B)
+    rows = size[0]
+    most = _most('paged_append', rows, B, cu, most)
+    for t in (pk, pv):
+        if (ps[0] > 1 and t[0] == 0) or (ps[1] > 1 and t[1] == 0) or t[2] == 0:
+            raise ValueError('paged_append: rows of the pages overlap (an expanded tensor)')
+    xk, xv, xt, xl, xs, xc, xpk, xpv = _ptrs('paged_append', k, v, table, lens, start, cu, *pages)
+    if most and rows:
+        rc = _lib.lib().tcq_paged_append(xk, sk[0], sk[1], xv, sv[0], sv[1], xc, rows, most, B, ps[1], ps[3], xpk, pk[0], pk[1], pk[2], xpv, pv[0], pv[1],
+                                         pv[2], ps[0], ps[2], xt, N, xl, xs, stream())
+        if rc:
+            _lib.failed('tcq_paged_append', rc)
+
+
+def _queries(what, q, Hk, D, dt, o):
+    """Sizes and strides of q (rows, Hq, D), and o."""
+    size, sq = q.shape, q.stride()
+    if not (len(size) == 3 and size[2] == D and sq[2] == 1 and size[1] > 0 and Hk > 0 and size[1] % Hk == 0):
+        raise ValueError(f'{what}: q must be (rows, a multiple of {Hk} heads, {D}) with contiguous values, got {tuple(size)}')
+    if q.dtype != dt or dt not in _PAGE_TYPES:
+        raise TypeError(f'{what}: q, k and v must be all bfloat16 or all float16, got {q.dtype} and {dt}')
+    if o is None:
+        o = torch.empty(size, dtype=dt, device=q.device)
+    elif o.shape != size or o.dtype != dt or not o.is_contiguous():
+        raise ValueError(f'{what}: o must be contiguous {tuple(size)} {dt}')
+    return size[0], size[1], sq[0] if size[0] > 1 else 0, sq[1] if size[1] > 1 else 0, o
+
+
+def paged_attend(q, pages, table, lens, o=None, causal=True, cu=None, most=None, scale=None, keys=None):
+    """Attention of q (rows, Hq, D; the pages' type, 16-byte aligned, strides multiples of 8) over the first lens[b] rows of every sequence in the
+    pages (one layer's, any strides that are multiples of 8) that table (B, N) names, Hq a multiple of their heads: o (rows, Hq, D). B equal
+    shares of the rows, or cu and most as in paged_append; causal, scale, keys and rows of no sequence as in kv8_attend."""
+    ps, pk, pv, dt = _one_layer(pages, 'paged_attend')
+    B, N = _tables('paged_attend', table, lens)
+    rows, Hq, qt, qh, o = _queries('paged_attend', q, ps[1], ps[3], dt, o)
+    most = _most('paged_attend', rows, B, cu, most)
+    xq, xl, xt, xc, xo, xk, xv = _ptrs('paged_attend', q, lens, table, cu, o, *pages)
+    if most and rows:
+        D, cap = ps[3], N * ps[2]
+        keys = cap if keys is None else max(0, min(int(keys), cap))
+        L = _lib.lib()
+        floats = L.tcq_paged_attend_floats(rows, most, B, Hq, ps[1], D, keys)
+        part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        rc = L.tcq_paged_attend(xq, qt, qh, DTYPE[dt], xc, xl, rows, most, B, Hq, ps[1], D, xk, pk[0], pk[1], pk[2], xv, pv[0], pv[1], pv[2], ps[0], ps[2],
+                                xt, N, causal, D ** -0.5 if scale is None else scale, keys, part.data_ptr() if floats else None, xo, stream())
+        if rc:
+            _lib.failed('tcq_paged_attend', rc)
+    return o
+
+
+class PagedRows:
+    """One layer's pages as a decoder layer takes them in the place of its key rows (gemma.PagedKVCache.rows): the call's rows are equal shares of the
+    table's sequences, or as cu and most say. core() puts them at positions start[b] .. of sequence b and attends over its first lens[b] rows, the
+    new ones with them (both (B,) int32 on the device; pages_take makes the room); a later call with the same start replaces them."""
+
+    def __init__(self, pages, table, lens, start, keys=None, cu=None, most=None):
+        self.pages, self.table, self.lens, self.start, self.keys, self.cu, self.most = pages, table, lens, start, keys, cu, most
+
+    def core(self, q, k, v, heads, causal):
+        """Attention of q (M, heads * D) after k, v (M, H * D): o (M, heads * D)."""
+        M, D = q.shape[0], self.pages.k.shape[-1]
+        paged_append(self.pages, k.reshape(M, -1, D), v.reshape(M, -1, D), self.table, self.lens, self.start, self.cu, self.most)
+        return paged_attend(q.reshape(M, heads, D), self.pages, self.table, self.lens, causal=causal, cu=self.cu, most=self.most,
+                            keys=self.keys).view(M, heads * D)
+
+
+def cross_attend(q, k, v, lens=None, mask=None, o=None, cu=None, most=None, scale=None):
+    """Attention of q (rows, Hq, D; BF16 / FP16, 16-byte aligned, strides multiples of 8) to an encoder's states of another length: k, v (B, T, H, D) of the
+    same type, 16-byte aligned, strides multiples of 8 (views into a product's rows), Hq a multiple of H. Every row of sequence b sees
+    keys 0 .. lens[b] - 1 (B, int32, on the device; None: all) with mask[b, j] (B, T, bool; None: all): o (rows, Hq, D), zeros where
+    that is none. B equal shares of the rows, or cu and most as in kv8_attend; scale: of the scores, 1 / sqrt(D) by default."""
+    ks, sk, sv, dt = k.shape, k.stride(), v.stride(), k.dtype
+    if not (len(ks) == 4 and ks == v.shape and v.dtype == dt and sk[3] == sv[3] == 1 and ks[0] > 0):
+        raise ValueError('cross_attend: k and v must be (sequences, keys, heads, D) of one type with contiguous values')
+    B, T, H, D = ks
+    rows, Hq, qt, qh, o = _queries('cross_attend', q, H, D, dt, o)
+    if lens is not None:
+        _counts('cross_attend', lens, B)
+    if mask is not None and not (mask.dtype == torch.bool and mask.shape == (B, T) and (mask.stride(1) == 1 or T < 2)):
+        raise ValueError(f'cross_attend: mask must be ({B}, {T}) bool with contiguous keys')
+    most = _most('cross_attend', rows, B, cu, most)
+    xq, xk, xv, xl, xm, xc, xo = _ptrs('cross_attend', q, k, v, lens, mask, cu, o)
+    if most and rows:
+        if T == 0:
+            raise ValueError('cross_attend: no keys')
+        L = _lib.lib()
+        floats = L.tcq_cross_attend_floats(rows, most, B, Hq, H, D, T)
+        part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+        rc = L.tcq_cross_attend(xq, qt, qh, DTYPE[dt], xc, rows, most, B, Hq, H, D, xk, sk[0], sk[2], sk[1], xv, sv[0], sv[2], sv[1], T, xl, xm,
+                                0 if mask is None else mask.stride(0), D ** -0.5 if scale is None else scale, part.data_ptr() if floats else None, xo,
+                                stream())
+        if rc:
+            _lib.failed('tcq_cross_attend', rc)
+    return o
+
+
 # ------------------------------------------------------------------------------------------------------------- attention
 def attend(q, k_cache, v_cache, k_new, v_new, heads, causal_offset=None, o=None, su=None, q8=None, scale=None, q4=None):
     """Multi-query attention (H <= 8 heads, head dim 256), BF16: keys / values = cache rows (or None) then the new rows.

@@ -666,7 +666,7 @@ class KDecoderLayer(torch.nn.Module):
             else:
                 STATS['chained_prologues'] += 1
             z1 = qkv.product(b)
-        in8 = isinstance(cache_k, kernels.KV8Rows)        # an 8-bit cache: its own append and attention, then the o projection's prologue
+        in8 = hasattr(cache_k, 'core')                    # an 8-bit cache, or pages: their own append and attention, then the o projection's prologue
         if not in8 and self._attn_post_fits(M, z1, qkv, og, cache_k, cache_v):
             # one token: the q/k/v epilogue runs inside the attention's launch (the query row never leaves it; the new key /
             # value rows go to kv_out), the chunk merge + o rotate + quantize inside the o product's launch
