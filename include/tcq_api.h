@@ -623,7 +623,7 @@ int tcq_paged_append(const void* k, int64_t k_tok, int64_t k_head, const void* v
                      tcq_stream_t stream);
 
 /* Softmax attention of q (rows, Hq, D), BF16 or FP16, D a multiple of 8 up to 256, over the first lens[b] rows of every sequence of such a cache (Hk
- * heads, Hq a multiple of Hk; q, k, v of one type; strides in elements, multiples of 8; 16-byte aligned): o (rows, Hq, D), contiguous. Rows of
+ * heads, Hq a multiple of Hk; q, k, v of one type; strides in elements, multiples of 8, a token's of at least D; 16-byte aligned): o (rows, Hq, D), contiguous. Rows of
  * sequence b: B equal shares of `most` rows, or rows cu[b] .. cu[b + 1] - 1, at most `most` of them. causal: row i of a sequence's n sees
  * positions up to lens[b] - n + i. A row that sees nothing is zeros; rows of no sequence are left as they are. An entry of the table outside the
  * pool counts as page 0. keys: about the longest length, for the split of the work alone. part: tcq_paged_attend_floats(...) floats of workspace

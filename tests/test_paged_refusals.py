@@ -36,7 +36,7 @@ BAD_ATTEND = [(dict(q=None), ARG), (dict(k=None), ARG), (dict(v=None), ARG), (di
               (dict(most=0), ARG), (dict(B=0), ARG), (dict(Hk=0), ARG), (dict(D=0), ARG), (dict(keys=-1), ARG), (dict(scale=-1.0), ARG),
               (dict(scale=float('nan')), ARG), (dict(scale=float('inf')), ARG), (dict(dtype=0), DTYPE), (dict(dtype=I8), DTYPE), (dict(Hk=3), SHAPE),
               (dict(cu=None, most=3), SHAPE), (dict(D=68), UNSUPPORTED), (dict(D=264), UNSUPPORTED), (dict(B=70000), UNSUPPORTED),
-              (dict(kt=1 << 25), UNSUPPORTED), (dict(vh=-64), UNSUPPORTED), (dict(qt=65), ALIGN), (dict(kt=60), ALIGN), (dict(q=P + 2), ALIGN),
+              (dict(kt=1 << 25), UNSUPPORTED), (dict(vh=-64), UNSUPPORTED), (dict(vt=56), UNSUPPORTED), (dict(qt=65), ALIGN), (dict(kt=68), ALIGN), (dict(q=P + 2), ALIGN),
               (dict(k=P + 8), ALIGN), (dict(o=P + 8), ALIGN), (dict(part=P + 4), ALIGN)]
 
 

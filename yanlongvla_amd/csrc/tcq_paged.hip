@@ -33,7 +33,7 @@ struct Attn {
     const int *cu, *lens;
     u16* o;
     float *part, *stat;                  // split: outputs (row, head, split, D) and maxima / sums (.., 2)
-    int rows, most, Hk, G, D, N, shift, pages, cap, causal, S, tiles;
+    int rows, most, Hk, G, D, N, shift, pages, cap, causal, S, tiles, sorted;
     float sl;
 };
 
@@ -96,6 +96,29 @@ __device__ __forceinline__ u32 out2(float a, float b) {
 __device__ __forceinline__ uint2_t read_tr(const char* p) {
     return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
 }
+// 2 or 4 pairs of transposing reads, of the rows at p[i] and SECOND bytes further, complete on return. The wait is in the same block; read_tr
+// instead makes the compiler wait for every load that was issued since one into the LDS, the next keys' among them.
+template <int N, int AT, int SECOND>
+__device__ __forceinline__ void read_tr_all(const int* p, uint4_t* v) {
+    static_assert(N == 2 || N == 4, "a block of reads");
+    uint2_t x[4], y[4];
+    if constexpr (N == 4)
+        asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%c12\n\tds_read_b64_tr_b16 %1, %8 offset:%c13\n\t"
+                     "ds_read_b64_tr_b16 %2, %9 offset:%c12\n\tds_read_b64_tr_b16 %3, %9 offset:%c13\n\t"
+                     "ds_read_b64_tr_b16 %4, %10 offset:%c12\n\tds_read_b64_tr_b16 %5, %10 offset:%c13\n\t"
+                     "ds_read_b64_tr_b16 %6, %11 offset:%c12\n\tds_read_b64_tr_b16 %7, %11 offset:%c13\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0]), "=&v"(y[0]), "=&v"(x[1]), "=&v"(y[1]), "=&v"(x[2]), "=&v"(y[2]), "=&v"(x[3]), "=&v"(y[3])
+                     : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(AT), "n"(AT + SECOND)
+                     : "memory");
+    else
+        asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%c6\n\tds_read_b64_tr_b16 %1, %4 offset:%c7\n\t"
+                     "ds_read_b64_tr_b16 %2, %5 offset:%c6\n\tds_read_b64_tr_b16 %3, %5 offset:%c7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0]), "=&v"(y[0]), "=&v"(x[1]), "=&v"(y[1])
+                     : "v"(p[0]), "v"(p[1]), "n"(AT), "n"(AT + SECOND)
+                     : "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = uint4_t{x[i][0], x[i][1], y[i][0], y[i][1]};
+}
 // at most vm loads (63: any) and lgkm LDS operations (15: any) still under way
 template <int vm, int lgkm>
 __device__ __forceinline__ void wait_for() {
@@ -103,13 +126,14 @@ __device__ __forceinline__ void wait_for() {
 }
 __device__ __forceinline__ void order() { asm volatile("" ::: "memory"); }
 
-// Rows of DP dims (RS bytes) in LDS: where the 16-byte piece p of key row r lies in its row. Keys are read 32 (16) rows at one piece,
-// values 4 rows at one pair of pieces a quarter wave.
+// Rows of DP dims (RS bytes) in LDS: the 16-byte piece p of row r lies at p ^ turn(r) of its row. A quarter wave reads one piece of 16 keys, half a wave
+// 64 bytes of 4 value rows (32 x 32 products: wide) or 32 bytes of 8 (16 x 16): no two on the same of the 64 banks.
 template <int DP>
 struct Place {
     static constexpr int RS = 2 * DP, PR = DP / 8, NI = PR / 4;          // bytes and pieces of a row, 1 KiB loads of 16 rows
     __device__ static int key(int r) { return DP == 64 ? (r >> 1) & 7 : DP == 96 ? (r >> 2) & 3 : r & 15; }
-    __device__ static int val(int r) { return DP == 64 ? (r & 6) : DP == 96 ? 0 : 2 * (r & 7); }
+    __device__ static int wide(int r) { return DP == 64 ? (2 * r) & 4 : DP == 96 ? 0 : 4 * (r & 3); }
+    __device__ static int val(int r) { return DP == 64 ? r & 6 : DP == 96 ? 0 : 2 * (r & 7); }
 };
 
 // What a workgroup's sequence is: its rows, keys and what its tokens see.
@@ -118,14 +142,14 @@ struct Seq {
     int n, cnt, len, end;                // processed and all new tokens, keys held, keys counted
     __device__ __forceinline__ int sees(int t, int causal) const { return causal ? max(0, min(len, end - cnt + t + 1)) : len; }
 };
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ Seq seq_of(const Attn& a, int b) {
     Seq s;
-    s.c0 = a.cu ? a.cu[b] : (int64_t)b * a.most;
-    s.cnt = a.cu ? a.cu[b + 1] - (int)s.c0 : a.most;
-    s.c0 = max((int64_t)0, min(s.c0, (int64_t)a.rows));
-    s.cnt = max(0, s.cnt);
-    s.n = (int)min((int64_t)min(s.cnt, a.most), a.rows - s.c0);
-    s.end = a.lens ? a.lens[b] : a.cap;
+    const int64_t c0 = a.cu ? a.cu[b] : (int64_t)b * a.most;
+    s.cnt = uniform(max(0, a.cu ? a.cu[b + 1] - (int)c0 : a.most));
+    s.c0 = uniform((int)max((int64_t)0, min(c0, (int64_t)a.rows)));
+    s.n = min(min(s.cnt, a.most), a.rows - (int)s.c0);
+    s.end = uniform(a.lens ? a.lens[b] : a.cap);
     s.len = max(0, min(s.end, a.cap));
     return s;
 }
@@ -152,83 +176,143 @@ struct Rows {
         return a.v + v0 + (PAGED ? page * a.vb + (p & ((1 << a.shift) - 1)) * a.vt : p * a.vt);
     }
 };
-constexpr u32 SPAN = 0x7ffffff0u;        // 16 rows from a base lie below 2 GiB
-// 16 bytes a lane at its offset from a uniform base: to LDS (lane l at dst + 16 l), or to registers
-__device__ __forceinline__ void row_to_lds(const char* base, u32 off, char* dst) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(base, SPAN), (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
+// 16 bytes a lane at its offset from a uniform base, zeros from `bytes` on. A token's row is no longer than the way to the next, so `bytes` of n
+// rows cuts off whole rows: those behind the last key need no test of their own. (The compiler must see that a descriptor is the same for the
+// wave, or it makes a loop over its lanes: hence uniform.)
+__device__ __forceinline__ rsrc_t rows_rsrc(const char* base, u32 bytes) {
+    const u64 p = (u64)base;
+    return make_rsrc((const void*)((u64)(u32)uniform((int)p) | (u64)(u32)uniform((int)(p >> 32)) << 32), (u32)uniform((int)bytes));
 }
-__device__ __forceinline__ uint4_t row_piece(const char* base, u32 off, int more) {
-    return __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(base, SPAN), off, more, 0));
+__device__ __forceinline__ uint4_t row_piece(const char* base, u32 bytes, u32 off, int more) {
+    return __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(base, bytes), off, more, 0));
+}
+__device__ __forceinline__ void row_to_lds(const char* base, u32 bytes, u32 off, char* dst) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rows_rsrc(base, bytes), (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
 }
 
 __device__ __forceinline__ u64 first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
+template <int N> using Num = std::integral_constant<int, N>;
+
+// Which tile of R rows of which sequence and head workgroup k takes: the k-th when they are ordered by the keys that they see (in steps of 64), the
+// most first, so that the last ones to start are short. A lane counts for one sequence (at most 64); found by bisection of the number of keys.
+struct Job {
+    int b, h, tile;
+};
+__device__ __forceinline__ int wave_total(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);
+    return __builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16) + __builtin_amdgcn_readlane(x, 32) + __builtin_amdgcn_readlane(x, 48);
+}
+__device__ __forceinline__ Job longest(const Attn& a, int B, int R, int k) {
+    const int lane = threadIdx.x & 63, b = min(lane, B - 1);
+    const int c0 = a.cu ? a.cu[b] : b * a.most, cnt = max(0, a.cu ? a.cu[b + 1] - c0 : a.most), at = max(0, min(c0, a.rows));
+    const int n = lane < B ? min(min(cnt, a.most), a.rows - at) : 0, end = a.lens ? a.lens[b] : a.cap, len = max(0, min(end, a.cap));
+    const int nrows = n * a.G, tiles = (nrows + R - 1) / R;
+    // tiles of the sequence that see at least x keys: the tokens from x - end + cnt - 1 on do, tile i ends with row R (i + 1) - 1
+    auto count = [&](int x) {
+        if (x <= 0) return tiles;
+        if (x > len) return 0;
+        if (!a.causal) return tiles;
+        const int t = max(0, x - end + cnt - 1);
+        return t >= n ? 0 : tiles - t * a.G / R;
+    };
+    int lo = 0, hi = (a.cap >> 6) + 1;                                   // the most steps that more than k tiles see
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (wave_total(count(64 * mid)) * a.Hk > k) lo = mid;
+        else hi = mid;
+    }
+    const int more = count(64 * (lo + 1)), same = count(64 * lo) - more;
+    int left = k - wave_total(more) * a.Hk, before = same;              // among those of `lo` steps, by sequence
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(before, d);
+        before += lane >= d ? y : 0;
+    }
+    before = (before - same) * a.Hk;
+    const u64 mine = __builtin_amdgcn_ballot_w64(same > 0 && before <= left);
+    if (left < 0 || !mine) return {0, 0, a.tiles};                       // (no such tile: past the rows of every sequence)
+    const int who = 63 - __builtin_clzll(mine);
+    left -= __builtin_amdgcn_readlane(before, who);
+    if (left >= __builtin_amdgcn_readlane(same, who) * a.Hk) return {0, 0, a.tiles};
+    return {who, left % a.Hk, __builtin_amdgcn_readlane(tiles - more, who) - 1 - left / a.Hk};
+}
+
 // ------------------------------------------------------------------------------------------------------------ many rows
-constexpr int rows_keys(int DP) { return DP == 256 ? 32 : 64; }      // keys of a tile
+constexpr int rows_keys(int DP) { return DP == 256 ? 32 : 64; }       // keys of a tile
 
 // W waves of 32 rows each; tiles of BK keys and values in LDS, the next tile's loads in flight behind one barrier a tile. Scores and
 // outputs on 32 x 32 x 16 products: row r of a wave is column r of S^T and O^T.
-template <int DP, bool BF, bool PAGED, int W>
+template <int DP, bool BF, bool PAGED, bool MASK, int W>
 __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
     using P = Place<DP>;
     constexpr int BK = rows_keys(DP), NK = BK / 32, KS = DP / 16, DT = DP / 32, HALF = BK * P::RS;   // (a tile's values lie HALF behind its keys)
-    constexpr int NG = BK / 16, NU = 2 * NG / W;                         // groups of 16 keys, and loads of 16 rows a wave
-    static_assert(2 * NG % W == 0, "every wave loads as much");
+    constexpr int NG = BK / 16, U = 2 * NG / W;                          // units of 16 rows of keys, then values; those of a wave
+    static_assert(U * W == 2 * NG, "every wave fetches as much");
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h2 = lane >> 5, r32 = lane & 31;
-    const int groups = gridDim.x / a.tiles, gi = blockIdx.x % groups, rt = a.tiles - 1 - blockIdx.x / groups;
-    const int s = gi % a.S, h = gi / a.S % a.Hk, b = gi / a.S / a.Hk;
+    const int groups = gridDim.x / a.tiles, gi = blockIdx.x % groups;
+    int s = 0, h, b, at_tile;
+    if (a.sorted) {
+        const Job x = longest(a, groups / a.Hk, 32 * W, blockIdx.x);
+        b = x.b, h = x.h, at_tile = x.tile;
+    } else {
+        s = gi % a.S, h = gi / a.S % a.Hk, b = gi / a.S / a.Hk;
+        at_tile = a.tiles - 1 - blockIdx.x / groups;
+    }
     const Seq sq = seq_of(a, b);
-    const int nrows = sq.n * a.G, row0 = rt * 32 * W;
+    constexpr int RW = 32;                                               // rows of a wave
+    const int nrows = sq.n * a.G, row0 = at_tile * RW * W;
     if (row0 >= nrows) return;
-    const int wrow = row0 + 32 * wave, row = wrow + r32, tok = min(row, nrows - 1) / a.G, hq = h * a.G + min(row, nrows - 1) - tok * a.G;
-    const int smax = sq.sees((min(row0 + 32 * W, nrows) - 1) / a.G, a.causal), nt = (smax + BK - 1) / BK;
-    const int wmax = wrow < nrows ? sq.sees((min(wrow + 32, nrows) - 1) / a.G, a.causal) : 0;
-    const int vend = row < nrows ? sq.sees(tok, a.causal) : 0;
+    const int wrow = row0 + RW * wave, smax = sq.sees((min(row0 + RW * W, nrows) - 1) / a.G, a.causal), nt = (smax + BK - 1) / BK;
     const int t0 = (int)((int64_t)nt * s / a.S), t1 = (int)((int64_t)nt * (s + 1) / a.S);
     const Rows<PAGED> at(a, b, h);
 
-    // the row's query, 16 bytes of dims 16 ks + 8 h2 .. a K step
+    // this lane's row: its place (row, head) in q and o, the keys that it sees, its query, 16 bytes of dims 16 ks + 8 h2 .. a K step
+    const int row = wrow + r32, some = min(row, nrows - 1), tok = some / a.G, hq = h * a.G + some - tok * a.G;
+    const int vend = row < nrows ? sq.sees(tok, a.causal) : 0;
     uint4_t Q[KS];
     {
         const u16* p = a.q + (sq.c0 + tok) * a.q_tok + hq * a.q_head + 8 * h2;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) Q[ks] = 16 * ks + 8 * h2 < a.D ? *gptr((const uint4_t*)(p + 16 * ks)) : uint4_t{0, 0, 0, 0};
     }
-    // offsets of this lane's pieces of 16 rows: piece L of the 16 rows' lies in LDS at 16 L
-    u32 ok[P::NI], ov[P::NI];
-#pragma unroll
-    for (int i = 0; i < P::NI; ++i) {
-        const int L = 64 * i + lane, r = L / P::PR, p = L - r * P::PR, pk = p ^ P::key(r), pv = p ^ P::val(r);
-        ok[i] = 8 * pk < a.D ? (u32)(r * a.kt) + 16 * pk : RSRC_OOB;
-        ov[i] = 8 * pv < a.D ? (u32)(r * a.vt) + 16 * pv : RSRC_OOB;
-    }
-    const uint8_t* mrow = !PAGED && a.mask ? a.mask + b * a.mask_b : nullptr;
+    // A wave fetches U units of 16 rows of a tile, P::NI loads of 1 KiB each, piece L of the rows at 16 L in LDS. Keys that no row sees are zeros:
+    // those behind the last one by the bound of the loads, masked ones (bits) lane by lane.
+    const uint8_t* mrow = MASK ? a.mask + b * a.mask_b : nullptr;
     auto mask_byte = [&](int j) { return lane < BK && BK * j + lane < smax ? (int)gptr(mrow)[BK * j + lane] : 0; };
-    // tile j's rows that some row sees (bits) to LDS; the others, which no row sees, are zeros there
-    auto issue = [&](int j, int buf, u64 bits, const int (&page)[NU]) {
-        if (!bits) return;
+    u32 off[U][P::NI];
 #pragma unroll
-        for (int x = 0; x < NU; ++x) {
-            const int u = wave + W * x, g = u % NG, p0 = BK * j + 16 * g;
-            const bool val = W <= NG ? W * x >= NG : u >= NG;            // uniform
-            char* dst = lds + buf * 2 * HALF + u * 16 * P::RS;
-            const u32 on = (u32)(bits >> (16 * g)) & 0xffffu;
-            const char* const base = val ? at.val(a, p0, page[x]) : at.key(a, p0, page[x]);
-            if (on == 0xffffu) {
+    for (int u = 0; u < U; ++u) {
+        const bool val = W > NG ? wave >= NG : W * u >= NG;              // unit u of the wave holds values (uniform)
 #pragma unroll
-                for (int i = 0; i < P::NI; ++i)
-                    row_to_lds(base, val ? ov[i] : ok[i], dst + i * 1024);
-            } else {
+        for (int i = 0; i < P::NI; ++i) {
+            const int L = 64 * i + lane, r = L / P::PR, p = (L - r * P::PR) ^ (val ? P::wide(r) : P::key(r));
+            off[u][i] = 8 * p < a.D ? (u32)(r * (val ? a.vt : a.kt)) + 16 * p : RSRC_OOB;
+        }
+    }
+    auto fetch = [&](int j, u64 bits, const int (&page)[U]) {
 #pragma unroll
-                for (int i = 0; i < P::NI; ++i)
-                    row_to_lds(base, (on >> ((64 * i + lane) / P::PR)) & 1 ? (val ? ov[i] : ok[i]) : RSRC_OOB, dst + i * 1024);
+        for (int u = 0; u < U; ++u) {
+            const bool val = W > NG ? wave >= NG : W * u >= NG;
+            const int g = (wave + W * u) % NG, p0 = BK * j + 16 * g;
+            const char* const base = val ? at.val(a, p0, page[u]) : at.key(a, p0, page[u]);
+            const u32 bytes = (u32)max(0, min(16, smax - p0)) * (u32)(val ? a.vt : a.kt);
+            char* const dst = lds + (2 * (j & 1) + (int)val) * HALF + g * 16 * P::RS;
+#pragma unroll
+            for (int i = 0; i < P::NI; ++i) {
+                u32 o = off[u][i];
+                if constexpr (MASK) o = (u32)(bits >> (16 * g)) >> ((64 * i + lane) / P::PR) & 1 ? o : RSRC_OOB;
+                row_to_lds(base, bytes, o, dst + i * 1024);
             }
         }
     };
-    auto pages_of = [&](int j, int (&page)[NU]) {
+    auto pages_of = [&](int j, int (&page)[U]) {
 #pragma unroll
-        for (int x = 0; x < NU; ++x) page[x] = at.page(a, BK * j + 16 * ((wave + W * x) % NG));
+        for (int u = 0; u < U; ++u) page[u] = at.page(a, BK * j + 16 * ((wave + W * u) % NG));
     };
     // byte offsets of the fragments in a tile: K step ks of the first 32 keys, dims 32 dt .. of the first 8 values (turns stay within 256 bytes)
     constexpr int FK = KS < 8 ? KS : 8, FV = DT < 4 ? DT : 4;
@@ -238,7 +322,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
     {
         const int i = lane & 15, r = 4 * h2 + (i >> 2);
 #pragma unroll
-        for (int dt = 0; dt < FV; ++dt) fv[dt] = HALF + r * P::RS + 16 * ((4 * dt + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ P::val(r)) + 8 * (i & 1);
+        for (int dt = 0; dt < FV; ++dt) fv[dt] = HALF + r * P::RS + 16 * ((4 * dt + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ P::wide(r)) + 8 * (i & 1);
     }
     float16_t O[DT];
 #pragma unroll
@@ -249,54 +333,54 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
     u32 odd = 0;
     const float thr = 8.f / a.sl;
 
-    int page[NU], mb = 0;
-    u64 next = 0;
-    auto bits_of = [&](int j) -> u64 {                                   // (mb: the mask's bytes of tile j)
-        const u64 in = first_bits(min(BK, smax - BK * j));
-        return !PAGED && mrow ? in & __builtin_amdgcn_ballot_w64(mb != 0) : in;
-    };
+    int page[U], mb = 0;                                                 // pages of the next tile
+    u64 b0 = 0, b1 = 0;                                                  // MASK: bits of tiles j, j + 1
     if (t0 < t1) {
+        if (MASK) {
+            b1 = __builtin_amdgcn_ballot_w64(mask_byte(t0) != 0);
+            mb = mask_byte(t0 + 1);
+        }
         pages_of(t0, page);
-        if (!PAGED && mrow) mb = mask_byte(t0);
-        next = bits_of(t0);
-        if (!PAGED && mrow) mb = mask_byte(t0 + 1);
-        issue(t0, 0, next, page);
+        fetch(t0, b1, page);
         pages_of(t0 + 1, page);
     }
-    auto step = [&](int j, auto edge) {                                  // edge: rows may see a part of the tile
+    // One tile, the next one's loads under way. edge: rows may see a part of it.
+    auto step = [&](int j, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
-        const int buf = (j - t0) & 1;
-        const u64 bits = next;
-        wait_for<0, 0>();                                                // this tile's loads, and the reads of the one before
+        wait_for<0, 0>();                                                // this wave's rows in LDS, and its reads of the tile before
         order();
         __builtin_amdgcn_s_barrier();
         order();
+        if (MASK) {
+            b0 = b1;
+            b1 = __builtin_amdgcn_ballot_w64(mb != 0);
+            mb = mask_byte(j + 2);
+        }
         if (j + 1 < t1) {
-            next = bits_of(j + 1);
-            if (!PAGED && mrow) mb = mask_byte(j + 2);
-            issue(j + 1, buf ^ 1, next, page);
+            fetch(j + 1, b1, page);
             pages_of(j + 2, page);
         }
-        const char* T = lds + buf * 2 * HALF;
-        if (EDGE ? !bits || BK * j >= wmax : wrow >= nrows) return;      // uniform
+        if (wrow >= nrows || (MASK && !b0)) return;                      // uniform: no rows, or no keys that count
+        const char* T = lds + (j & 1) * 2 * HALF;
         float16_t S[NK];
 #pragma unroll
-        for (int kt = 0; kt < NK; ++kt) {
+        for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) S[kt][e] = 0.f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) S[kt] = mma32<BF>(*(const uint4_t*)(T + fk[ks % FK] + 256 * (ks / FK) + kt * 32 * P::RS), Q[ks], S[kt]);
-        }
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < NK; ++kt) S[kt] = mma32<BF>(*(const uint4_t*)(T + fk[ks % FK] + 256 * (ks / FK) + kt * 32 * P::RS), Q[ks], S[kt]);
         float mx = LOWEST;
-        if constexpr (EDGE) {
-            const u64 mine = PAGED ? first_bits(min(BK, vend - BK * j)) : vend > BK * j ? bits : 0ull;
+        if (EDGE && (!MASK || b0 != first_bits(BK))) {                   // uniform (a mask is the same for all rows)
+            const u64 mine = MASK ? b0 : first_bits(min(BK, vend - BK * j));
             if (!mine) mx = -__builtin_inff();
-            const u64 w = mine >> (4 * h2);
+            const u64 x = mine >> (4 * h2);
 #pragma unroll
             for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    S[kt][e] = ((u32)(w >> (32 * kt)) >> (8 * (e >> 2) + (e & 3))) & 1 ? S[kt][e] : -__builtin_inff();
+                    S[kt][e] = ((u32)(x >> (32 * kt)) >> (8 * (e >> 2) + (e & 3))) & 1 ? S[kt][e] : -__builtin_inff();
         }
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt)
@@ -317,30 +401,28 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
         for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const u32 w = prob2<BF>(__builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][e], a.sl, -mc)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][e + 1], a.sl, -mc)));
-                l = sum2<BF>(w, l);
-                Pr[2 * kt + (e >> 3)][(e >> 1) & 3] = w;
+                const u32 x = prob2<BF>(__builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][e], a.sl, -mc)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][e + 1], a.sl, -mc)));
+                l = sum2<BF>(x, l);
+                Pr[2 * kt + (e >> 3)][(e >> 1) & 3] = x;
             }
         __builtin_amdgcn_sched_barrier(0);                               // (the values' reads no earlier: they take the scores' registers)
-        auto values = [&](int c, int dt) {
-            const char* p = T + fv[dt % FV] + 256 * (dt / FV) + c * 16 * P::RS;
-            const uint2_t x = read_tr(p), y = read_tr(p + 8 * P::RS);
-            return uint4_t{x[0], x[1], y[0], y[1]};
-        };
 #pragma unroll
         for (int c = 0; c < 2 * NK; ++c)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                if constexpr (EDGE && PAGED) O[dt] = mma32<BF>(finite<BF>(values(c, dt), odd), Pr[c], O[dt]);
-                else O[dt] = mma32<BF>(values(c, dt), Pr[c], O[dt]);
+                const char* p = T + fv[dt % FV] + 256 * (dt / FV) + c * 16 * P::RS;
+                const uint2_t x = read_tr(p), y = read_tr(p + 8 * P::RS);
+                uint4_t v = uint4_t{x[0], x[1], y[0], y[1]};
+                if constexpr (EDGE && PAGED) v = finite<BF>(v, odd);
+                O[dt] = mma32<BF>(v, Pr[c], O[dt]);
             }
     };
     // the tiles that all rows see in full, and those that they may see in part
-    const int tf = !PAGED && mrow ? t0 : max(t0, min(t1, sq.sees(row0 / a.G, a.causal) / BK));
+    const int tf = MASK ? t0 : max(t0, min(t1, sq.sees(row0 / a.G, a.causal) / BK));
     for (int j = t0; j < tf; ++j) step(j, std::false_type{});
     for (int j = tf; j < t1; ++j) step(j, std::true_type{});
     if (PAGED && __builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, false)) {   // uniform
-        const int last = min(BK * t1, wmax);
+        const int last = min(BK * t1, smax);
         for (int p = tf * BK; p < last; ++p) {
             const char* v = at.val(a, p, at.page(a, p)) + 8 * h2;
 #pragma unroll
@@ -356,7 +438,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
         }
     }
     l += lane_xor(l, 32, lane);
-    if (row >= nrows) return;
+    if (row >= nrows) return;                                            // (the lanes of a row go together)
     const int64_t out = (sq.c0 + tok) * (int64_t)(a.Hk * a.G) + hq;
     if (a.S > 1) {
         float* p = a.part + (out * a.S + s) * a.D;
@@ -421,29 +503,32 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
         ov[i] = 8 * pv < a.D ? (u32)(r * a.vt) + 16 * pv : RSRC_OOB;
     }
     const u32 ok = (u32)(lr * a.kt) + 16 * lg;
-    int fv[DT];
+    constexpr int FV = DT < 8 ? DT : 8;                                  // (turns stay within 256 bytes)
+    int fv[FV];                                                          // LDS addresses of dims 16 dt .. of the first 16 values
     {
-        const int r = 4 * lg + (lr >> 2);
+        const int r = 4 * lg + (lr >> 2), base = (int)(uintptr_t)(__attribute__((address_space(3))) const char*)T;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) fv[dt] = r * P::RS + 16 * ((2 * dt + ((lr >> 1) & 1)) ^ P::val(r)) + 8 * (lr & 1);
+        for (int dt = 0; dt < FV; ++dt) fv[dt] = base + r * P::RS + 16 * ((2 * dt + ((lr >> 1) & 1)) ^ P::val(r)) + 8 * (lr & 1);
     }
     uint4_t K[2][KS];
     auto load_k = [&](int j, u32 bits, const int (&page)[2]) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const char* const base = at.key(a, 32 * j + 16 * g, page[g]);
+            const u32 bytes = 0x7ffffff0u;
             const u32 off = (bits >> (16 * g + lr)) & 1 ? ok : RSRC_OOB;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) K[g][ks] = row_piece(base, 32 * ks + 8 * lg < a.D ? off : RSRC_OOB, 64 * ks);
+            for (int ks = 0; ks < KS; ++ks) K[g][ks] = row_piece(base, bytes, 32 * ks + 8 * lg < a.D ? off : RSRC_OOB, 64 * ks);
         }
     };
     auto load_v = [&](int j, u32 bits, const int (&page)[2]) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const char* const base = at.val(a, 32 * j + 16 * g, page[g]);
+            const u32 bytes = 0x7ffffff0u;
 #pragma unroll
             for (int i = 0; i < P::NI; ++i)
-                row_to_lds(base, (bits >> (16 * g + orow[i])) & 1 ? ov[i] : RSRC_OOB, T + g * 16 * P::RS + i * 1024);
+                row_to_lds(base, bytes, (bits >> (16 * g + orow[i])) & 1 ? ov[i] : RSRC_OOB, T + g * 16 * P::RS + i * 1024);
         }
     };
     auto bits_of = [&](int j) -> u32 {                                   // keys of tile j < t1 that any row may see
@@ -521,11 +606,19 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
             wait_for<63, 0>();
             order();
         }
+        auto product = [&](auto first, auto count) {                     // tiles of 16 dims
+            constexpr int dt = decltype(first)::value, N = decltype(count)::value;
+            if constexpr (dt < DT) {
+                uint4_t v[N];
+                read_tr_all<N, 256 * (dt / FV), 16 * P::RS>(fv + dt % FV, v);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const uint2_t x = read_tr(T + fv[dt]), y = read_tr(T + fv[dt] + 16 * P::RS);
-            O[dt] = mma16<BF>(uint4_t{x[0], x[1], y[0], y[1]}, Pr, O[dt]);
-        }
+                for (int i = 0; i < N; ++i) O[dt + i] = mma16<BF>(v[i], Pr, O[dt + i]);
+            }
+        };
+        product(Num<0>{}, Num<4>{});
+        product(Num<4>{}, Num<DT == 6 ? 2 : 4>{});
+        product(Num<8>{}, Num<4>{});
+        product(Num<12>{}, Num<4>{});
         wait_for<63, 0>();                                               // the next values take the place of these
         order();
     }
@@ -578,38 +671,64 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     }
 }
 
-// The parts of a row joined: thread (row and head, 4 dims), grid (most * Hq * D / 4 threads, B).
-template <bool BF>
+// The parts of a row joined: 64 threads for a row and head (4 dims each) and NG of them side by side over its parts, 4 / NG rows a workgroup; grid (rows,
+// B). Weights first (they are few), then the parts' outputs, eight loads under way.
+constexpr int MAX_PARTS = 64;        // one a lane
+template <bool BF, int NG>
 __global__ __launch_bounds__(256) void k_attend_join(Attn a) {
+    __shared__ float4_t sums[4][64];
     const Seq sq = seq_of(a, blockIdx.y);
-    const int D4 = a.D >> 2, Hq = a.Hk * a.G;
-    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, x = u / D4;
-    if (x >= (int64_t)sq.n * Hq) return;
-    const int d = 4 * (int)(u - x * D4);
-    const int64_t out = sq.c0 * Hq + x;
+    const int Hq = a.Hk * a.G, d = threadIdx.x & 63, wave = threadIdx.x >> 6, g = wave % NG;
+    const int64_t x = (int64_t)blockIdx.x * (4 / NG) + wave / NG;
+    const bool on = x < (int64_t)sq.n * Hq && 4 * d < a.D;
+    const int64_t out = sq.c0 * Hq + (x < (int64_t)sq.n * Hq ? x : 0);
     const float* st = a.stat + out * a.S * 2;
-    const float* p = a.part + out * a.S * a.D + d;
-    float M = -__builtin_inff(), L = 0.f;
-    for (int i = 0; i < a.S; ++i) M = fmaxf(M, gptr(st)[2 * i]);
-    float4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.S; ++i) {
-        const float mi = gptr(st)[2 * i], w = mi == -__builtin_inff() ? (M == mi ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mi - M);
-        L = __builtin_fmaf(w, gptr(st)[2 * i + 1], L);
-        v += *gptr((const float4_t*)(p + (int64_t)i * a.D)) * w;
+    const float* p = a.part + out * a.S * a.D + 4 * d;
+    float mi = -__builtin_inff(), li = 0.f;                              // part d of the row's (at most 64)
+    if (d < a.S) {
+        const float2_t v = *gptr((const float2_t*)(st + 2 * d));
+        mi = v[0];
+        li = v[1];
     }
+    const float M = wave_max(mi), w = mi == -__builtin_inff() ? (M == mi ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mi - M), L = wave_sum(d < a.S ? w * li : 0.f);
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int i = g; i < a.S; i += NG) {
+        const float wi = lane_value(w, i);
+        if (on) v += *gptr((const float4_t*)(p + (int64_t)i * a.D)) * wi;
+    }
+    if constexpr (NG > 1) {
+        sums[wave][d] = v;
+        __syncthreads();
+        if (g) return;
+#pragma unroll
+        for (int k = 1; k < NG; ++k) v += sums[wave + k][d];
+    }
+    if (!on) return;
     v *= M == -__builtin_inff() && L == 0.f ? 0.f : 1.f / L;
-    *gptr((uint2_t*)(a.o + out * a.D + d)) = uint2_t{out2<BF>(v[0], v[1]), out2<BF>(v[2], v[3])};
+    *gptr((uint2_t*)(a.o + out * a.D + 4 * d)) = uint2_t{out2<BF>(v[0], v[1]), out2<BF>(v[2], v[3])};
 }
 
+// How a call is split: which kernel, and the parts S of the keys (tiles of 64 of them).
+//   Few rows: up to 32 of a KV head (its 16-row workgroups read every key once, or twice), and calls whose rows make no more than 320 such workgroups
+//   over at most 16 tiles: their four waves share the keys of a row, where the other kernel would need parts and their join (50 rows of 32 heads x 48 to
+//   600 keys 6.6 us against 10.0, 300 x 300 of 16 x 64 7.1 against 10.4, 8 x 50 rows of 8 heads on 1 x 256 behind 850 22.9 against 27.4; 4000 keys 83
+//   against 46).
+//   Parts: as many as fill the chip, of one tile (the other kernel: two) or more. Few rows take 1024 workgroups (32 sequences of 16 heads on 8 x 128 behind
+//   4 to 8 thousand keys 176 us, 512: 203, 2048: 179), but 16 and more rows a workgroup, whose parts are larger to write and to join, 512 over many
+//   tiles (4 x 16 rows behind 8000 keys 42.6, 1024: 53) and 256 over few. No parts where they save less than their join takes, about 4 us, at
+//   D / 200 us a tile.
+//   (Times in a captured graph, joins included.)
 struct Plan {
     int few, S;
 };
 Plan plan_of(int B, int most, int G, int Hk, int D, int keys) {
-    const int64_t n = (int64_t)most * G, heads = (int64_t)B * Hk;
-    const int few = n <= 32;
-    const int64_t groups = heads * (few ? (n + 15) / 16 : (n + 127) / 128), tiles = ((int64_t)keys + 63) / 64;
-    const int64_t want = few ? 1024 : 512;
-    const int64_t S = max((int64_t)1, min(min(want / groups, tiles / (few ? 4 : 4)), (int64_t)64));
+    const int64_t n = (int64_t)most * G, heads = (int64_t)B * Hk, tiles = ((int64_t)keys + 63) / 64;
+    const bool few = n <= 32 || (heads * ((n + 15) / 16) <= 320 && tiles <= 16);
+    const int64_t groups = heads * (few ? (n + 15) / 16 : (n + 127) / 128);
+    const int64_t want = !few ? 512 : n < 16 ? 1024 : tiles >= 64 ? 512 : 256;
+    int64_t S = max((int64_t)1, min(min(want / groups, tiles / (few && n < 16 ? 1 : 2)), (int64_t)MAX_PARTS));
+    if (few && (tiles - tiles / S) * D < 800) S = 1;
     return {few, (int)S};
 }
 int64_t floats_of(int rows, int most, int B, int Hq, int Hk, int D, int keys) {
@@ -622,14 +741,19 @@ template <int DP, bool BF, bool PAGED>
 int run_dim(Attn& a, const Plan& p, int B, hipStream_t st) {
     const int64_t n = (int64_t)a.most * a.G;
     if (p.few) {
-        constexpr int W = 4;
         a.tiles = (int)((n + 15) / 16);
+        const dim3 grid((u32)((int64_t)a.tiles * a.S * a.Hk * B));
+        constexpr int W = 4;
         const size_t lds = max((size_t)W * 32 * Place<DP>::RS, (size_t)W * 16 * (DP + 4 + 2) * 4);
-        launch_k(k_attend_few<DP, BF, PAGED, W>, dim3((u32)((int64_t)a.tiles * a.S * a.Hk * B)), dim3(64 * W), lds, st, a);
+        launch_k(k_attend_few<DP, BF, PAGED, W>, grid, dim3(64 * W), lds, st, a);
     } else {
         constexpr int W = 4;
         a.tiles = (int)((n + 32 * W - 1) / (32 * W));
-        launch_k(k_attend_rows<DP, BF, PAGED, W>, dim3((u32)((int64_t)a.tiles * a.S * a.Hk * B)), dim3(64 * W), (size_t)4 * rows_keys(DP) * Place<DP>::RS, st, a);
+        const int64_t grid = (int64_t)a.tiles * a.S * a.Hk * B;
+        const size_t lds = (size_t)4 * rows_keys(DP) * Place<DP>::RS;
+        a.sorted = a.S == 1 && B <= 64 && grid > 512 && (a.causal || B > 1);
+        if (!PAGED && a.mask) launch_k(k_attend_rows<DP, BF, false, true, W>, dim3((u32)grid), dim3(64 * W), lds, st, a);
+        else launch_k(k_attend_rows<DP, BF, PAGED, false, W>, dim3((u32)grid), dim3(64 * W), lds, st, a);
     }
     return launch_status();
 }
@@ -652,9 +776,16 @@ int run(Attn& a, bool bf, bool paged, int B, int keys, float* part, hipStream_t 
     else ATTEND(256);
 #undef ATTEND
     if (e || a.S <= 1) return e;
-    const dim3 grid((u32)(((int64_t)a.most * Hq * (a.D / 4) + 255) / 256), B);
-    if (bf) launch_k(k_attend_join<true>, grid, dim3(256), 0, st, a);
-    else launch_k(k_attend_join<false>, grid, dim3(256), 0, st, a);
+    const int64_t rows = (int64_t)a.most * Hq;
+#define JOIN(NG)                                                                                                        \
+    do {                                                                                                                \
+        const dim3 grid((u32)((rows + 4 / NG - 1) / (4 / NG)), B);                                                      \
+        if (bf) launch_k(k_attend_join<true, NG>, grid, dim3(256), 0, st, a);                                           \
+        else launch_k(k_attend_join<false, NG>, grid, dim3(256), 0, st, a);                                             \
+    } while (0)
+    if (a.S > 8) JOIN(4);
+    else JOIN(1);
+#undef JOIN
     return launch_status();
 }
 
@@ -667,9 +798,9 @@ int refuse(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_
     if (dtype != TCQ_BF16 && dtype != TCQ_F16) return TCQ_ERR_DTYPE;
     if (Hq % Hk || (!cu && (int64_t)most * B > rows)) return TCQ_ERR_SHAPE;
     if (D > 256 || D % 8 || B > 65535 || Hk > 65535) return TCQ_ERR_UNSUPPORTED;
-    if (min(min(min(q_tok, q_head), min(kb, kh)), min(min(kt, vb), min(vh, vt))) < 0 || max(kt, vt) >= (1 << 25)) return TCQ_ERR_UNSUPPORTED;
+    if (min(min(min(q_tok, q_head), min(kb, kh)), min(min(kt, vb), min(vh, vt))) < 0 || max(kt, vt) >= (1 << 25) || min(kt, vt) < D) return TCQ_ERR_UNSUPPORTED;
     const int64_t n = (int64_t)most * (Hq / Hk);
-    if (n > MANY - 256 || (int64_t)rows * Hq > MANY || (n / 16 + 1) * 64 * Hk > MANY / B || (n * Hk / 256 + 1) * (D / 4) > MANY) return TCQ_ERR_UNSUPPORTED;
+    if (n > MANY - 256 || (int64_t)rows * Hq > MANY || (n / 16 + 1) * 64 * Hk > MANY / B || (int64_t)most * Hq > MANY) return TCQ_ERR_UNSUPPORTED;
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 16 || (q_tok | q_head | kb | kh | kt | vb | vh | vt) % 8) return TCQ_ERR_ALIGN;
     return 0;
 }

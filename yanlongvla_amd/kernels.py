@@ -808,7 +808,8 @@ def cross_attend(q, k, v, lens=None, mask=None, o=None, cu=None, most=None, scal
         L = _lib.lib()
         floats = L.tcq_cross_attend_floats(rows, most, B, Hq, H, D, T)
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-        rc = L.tcq_cross_attend(xq, qt, qh, DTYPE[dt], xc, rows, most, B, Hq, H, D, xk, sk[0], sk[2], sk[1], xv, sv[0], sv[2], sv[1], T, xl, xm,
+        kt, vt = (sk[1], sv[1]) if T > 1 else (D, D)
+        rc = L.tcq_cross_attend(xq, qt, qh, DTYPE[dt], xc, rows, most, B, Hq, H, D, xk, sk[0], sk[2], kt, xv, sv[0], sv[2], vt, T, xl, xm,
                                 0 if mask is None else mask.stride(0), D ** -0.5 if scale is None else scale, part.data_ptr() if floats else None, xo,
                                 stream())
         if rc:
