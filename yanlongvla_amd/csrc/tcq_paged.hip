@@ -267,7 +267,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
     constexpr int RW = 32;                                               // rows of a wave
     const int nrows = sq.n * a.G, row0 = at_tile * RW * W;
     if (row0 >= nrows) return;
-    const int wrow = row0 + RW * wave, smax = sq.sees((min(row0 + RW * W, nrows) - 1) / a.G, a.causal), nt = (smax + BK - 1) / BK;
+    // (tiles that are not full leave waves without rows: not always on the same SIMD)
+    const int wrow = row0 + RW * ((wave + blockIdx.x + (blockIdx.x >> 8)) % W), smax = sq.sees((min(row0 + RW * W, nrows) - 1) / a.G, a.causal), nt = (smax + BK - 1) / BK;
     const int t0 = (int)((int64_t)nt * s / a.S), t1 = (int)((int64_t)nt * (s + 1) / a.S);
     const Rows<PAGED> at(a, b, h);
 
