@@ -43,7 +43,7 @@ BAD_ATTEND = [(dict(q=None), ARG), (dict(k=None), ARG), (dict(v=None), ARG), (di
 @pytest.mark.parametrize('name,good,bad', [
     ('tcq_pages_take', dict(**BOOK, take=P, start=P, **POOL, moves=P, stream=None),
      BAD_BOOK + BAD_POOL + [(dict(take=None), ARG), (dict(start=None), ARG), (dict(moves=None), ARG)]),
-    ('tcq_pages_fork', dict(**BOOK, src=P, dst=P, n=1, stream=None), BAD_BOOK + [(dict(src=None), ARG), (dict(dst=None), ARG), (dict(n=0), ARG)]),
+    ('tcq_pages_fork', dict(**BOOK, src=P, dst=P, n=1, stream=None), BAD_BOOK + [(dict(src=None), ARG), (dict(dst=None), ARG), (dict(n=0), ARG), (dict(n=65536), UNSUPPORTED)]),
     ('tcq_pages_trim', dict(**BOOK, keep=P, stream=None), BAD_BOOK + [(dict(keep=None), ARG)]),
     ('tcq_pages_compact', dict(**BOOK, **POOL, moves=P, stream=None), BAD_BOOK + BAD_POOL + [(dict(moves=None), ARG)]),
     ('tcq_pages_copy', dict(k=P, v=P, layers=1, pages=8, size=512, src=P, dst=P, n=1, stream=None),
@@ -109,7 +109,7 @@ def test_helpers_refuse():
     cases = [
         (V, lambda: K.pages_take(pt._replace(lens=ints(0)), pool, ints(1, 1))), (V, lambda: K.pages_take(pt, pool, ints(1))),
         (V, lambda: K.pages_take(pt, pool, ints(1, 1).long())), (V, lambda: K.pages_take(pt, K.kv_pages(9, 2, 64, 'cpu', 16), ints(1, 1))),
-        (V, lambda: K.pages_take(pt, K.kv_pages(8, 2, 64, 'cpu', 32), ints(1, 1))), (V, lambda: K.pages_take(pt, pool, ints(1, 1), start=ints(1))),
+        (V, lambda: K.pages_take(pt, K.kv_pages(8, 2, 64, 'cpu', 32), ints(1, 1))), (V, lambda: K.pages_take(pt, pool, ints(1, 1), start=ints(1))), (V, lambda: K.pages_take(pt, pool, ints(1, 1), start=pt.lens)),
         (V, lambda: K.pages_take(pt._replace(free=ints(0, 0)), pool, ints(1, 1))), (V, lambda: K.pages_fork(pt, ints(0, 1), ints(1))),
         (V, lambda: K.pages_trim(pt, ints(0))), (V, lambda: K.pages_compact(pt, K.Pages(pool.k.transpose(0, 1), pool.v.transpose(0, 1)))),
         (V, lambda: K.pages_copy(K.Pages(pool.k[0, 0], pool.v[0, 0]), ints(0), ints(1))), (V, lambda: K.pages_copy(pool, ints(0), ints(1, 2))),

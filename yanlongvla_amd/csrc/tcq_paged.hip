@@ -52,7 +52,7 @@ __device__ __forceinline__ float4_t mma16(uint4_t a, uint4_t b, float4_t c) {
 // takes the same values, so the shift cancels and what remains is as large as that of the nearest ones.
 template <bool BF>
 __device__ __forceinline__ u32 prob2(float a, float b) {
-    return BF ? bf16_cvt2(a, b) : __builtin_bit_cast(u32, __builtin_amdgcn_cvt_pkrtz(a, b));
+    return BF ? bf16_cvt2(a, b) : __builtin_bit_cast(u32, __builtin_convertvector(float2_t{a, b}, half2_t));
 }
 template <bool BF>
 __device__ __forceinline__ float sum2(u32 w, float c) {
@@ -95,29 +95,6 @@ __device__ __forceinline__ u32 out2(float a, float b) {
 // 4 x 16 transposing read: lane i of 16 gets column i of the rows that lanes 4 r .. 4 r + 3 name in 8-byte pieces
 __device__ __forceinline__ uint2_t read_tr(const char* p) {
     return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
-}
-// 2 or 4 pairs of transposing reads, of the rows at p[i] and SECOND bytes further, complete on return. The wait is in the same block; read_tr
-// instead makes the compiler wait for every load that was issued since one into the LDS, the next keys' among them.
-template <int N, int AT, int SECOND>
-__device__ __forceinline__ void read_tr_all(const int* p, uint4_t* v) {
-    static_assert(N == 2 || N == 4, "a block of reads");
-    uint2_t x[4], y[4];
-    if constexpr (N == 4)
-        asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%c12\n\tds_read_b64_tr_b16 %1, %8 offset:%c13\n\t"
-                     "ds_read_b64_tr_b16 %2, %9 offset:%c12\n\tds_read_b64_tr_b16 %3, %9 offset:%c13\n\t"
-                     "ds_read_b64_tr_b16 %4, %10 offset:%c12\n\tds_read_b64_tr_b16 %5, %10 offset:%c13\n\t"
-                     "ds_read_b64_tr_b16 %6, %11 offset:%c12\n\tds_read_b64_tr_b16 %7, %11 offset:%c13\n\ts_waitcnt lgkmcnt(0)"
-                     : "=&v"(x[0]), "=&v"(y[0]), "=&v"(x[1]), "=&v"(y[1]), "=&v"(x[2]), "=&v"(y[2]), "=&v"(x[3]), "=&v"(y[3])
-                     : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(AT), "n"(AT + SECOND)
-                     : "memory");
-    else
-        asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%c6\n\tds_read_b64_tr_b16 %1, %4 offset:%c7\n\t"
-                     "ds_read_b64_tr_b16 %2, %5 offset:%c6\n\tds_read_b64_tr_b16 %3, %5 offset:%c7\n\ts_waitcnt lgkmcnt(0)"
-                     : "=&v"(x[0]), "=&v"(y[0]), "=&v"(x[1]), "=&v"(y[1])
-                     : "v"(p[0]), "v"(p[1]), "n"(AT), "n"(AT + SECOND)
-                     : "memory");
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = uint4_t{x[i][0], x[i][1], y[i][0], y[i][1]};
 }
 // at most vm loads (63: any) and lgkm LDS operations (15: any) still under way
 template <int vm, int lgkm>
@@ -372,6 +349,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int kt = 0; kt < NK; ++kt) S[kt] = mma32<BF>(*(const uint4_t*)(T + fk[ks % FK] + 256 * (ks / FK) + kt * 32 * P::RS), Q[ks], S[kt]);
+        __builtin_amdgcn_s_setprio(0);                                   // (products before the other wave's vector instructions)
         float mx = LOWEST;
         if (EDGE && (!MASK || b0 != first_bits(BK))) {                   // uniform (a mask is the same for all rows)
             const u64 mine = MASK ? b0 : first_bits(min(BK, vend - BK * j));
@@ -406,6 +384,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
                 l = sum2<BF>(x, l);
                 Pr[2 * kt + (e >> 3)][(e >> 1) & 3] = x;
             }
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);                               // (the values' reads no earlier: they take the scores' registers)
 #pragma unroll
         for (int c = 0; c < 2 * NK; ++c)
@@ -496,28 +475,28 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     }
     char* const T = lds + wave * 32 * P::RS;
     u32 ov[P::NI];
-    int orow[P::NI];
 #pragma unroll
     for (int i = 0; i < P::NI; ++i) {
         const int L = 64 * i + lane, r = L / P::PR, p = L - r * P::PR, pv = p ^ P::val(r);
-        orow[i] = r;
         ov[i] = 8 * pv < a.D ? (u32)(r * a.vt) + 16 * pv : RSRC_OOB;
     }
     const u32 ok = (u32)(lr * a.kt) + 16 * lg;
     constexpr int FV = DT < 8 ? DT : 8;                                  // (turns stay within 256 bytes)
-    int fv[FV];                                                          // LDS addresses of dims 16 dt .. of the first 16 values
+    int fv[FV];                                                          // byte offsets of dims 16 dt .. of the first 16 values
     {
-        const int r = 4 * lg + (lr >> 2), base = (int)(uintptr_t)(__attribute__((address_space(3))) const char*)T;
+        const int r = 4 * lg + (lr >> 2);
 #pragma unroll
-        for (int dt = 0; dt < FV; ++dt) fv[dt] = base + r * P::RS + 16 * ((2 * dt + ((lr >> 1) & 1)) ^ P::val(r)) + 8 * (lr & 1);
+        for (int dt = 0; dt < FV; ++dt) fv[dt] = r * P::RS + 16 * ((2 * dt + ((lr >> 1) & 1)) ^ P::val(r)) + 8 * (lr & 1);
     }
+    const int j1 = min(smax, 32 * t1);                                   // (no keys past the last tile)
     uint4_t K[2][KS];
+    // keys that no row sees are zeros: in pages, those behind the last one, by the bound of the loads; of states, bits says which, lane by lane
+    auto bytes_of = [&](int p0, int64_t step) { return PAGED ? (u32)max(0, min(16, j1 - p0)) * (u32)step : 16 * (u32)step; };
     auto load_k = [&](int j, u32 bits, const int (&page)[2]) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const char* const base = at.key(a, 32 * j + 16 * g, page[g]);
-            const u32 bytes = 0x7ffffff0u;
-            const u32 off = (bits >> (16 * g + lr)) & 1 ? ok : RSRC_OOB;
+            const u32 bytes = bytes_of(32 * j + 16 * g, a.kt), off = PAGED || (bits >> (16 * g + lr)) & 1 ? ok : RSRC_OOB;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) K[g][ks] = row_piece(base, bytes, 32 * ks + 8 * lg < a.D ? off : RSRC_OOB, 64 * ks);
         }
@@ -526,10 +505,10 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const char* const base = at.val(a, 32 * j + 16 * g, page[g]);
-            const u32 bytes = 0x7ffffff0u;
+            const u32 bytes = bytes_of(32 * j + 16 * g, a.vt);
 #pragma unroll
             for (int i = 0; i < P::NI; ++i)
-                row_to_lds(base, bytes, (bits >> (16 * g + orow[i])) & 1 ? ov[i] : RSRC_OOB, T + g * 16 * P::RS + i * 1024);
+                row_to_lds(base, bytes, PAGED || (bits >> (16 * g + (64 * i + lane) / P::PR)) & 1 ? ov[i] : RSRC_OOB, T + g * 16 * P::RS + i * 1024);
         }
     };
     auto bits_of = [&](int j) -> u32 {                                   // keys of tile j < t1 that any row may see
@@ -547,8 +526,8 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     int j = t0 + wave, page[2];
     u32 bits = bits_of(j);
 #pragma unroll
-    for (int g = 0; g < 2; ++g) page[g] = j < t1 ? at.page(a, 32 * j + 16 * g) : 0;
-    load_k(j < t1 ? j : 0, bits, page);
+    for (int g = 0; g < 2; ++g) page[g] = at.page(a, 32 * j + 16 * g);
+    load_k(j, bits, page);
     for (; j < t1; j += W) {
         load_v(j, bits, page);
         order();
@@ -560,7 +539,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
             for (int ks = 0; ks < KS; ++ks) S[g] = mma16<BF>(K[g][ks], Q[ks], S[g]);
         }
         const u32 now = bits;
-        const int jn = j + W < t1 ? j + W : 0;                           // (past the last tile the loads read zeros)
+        const int jn = j + W;                                            // (past the last tile the loads read zeros)
         bits = bits_of(j + W);
 #pragma unroll
         for (int g = 0; g < 2; ++g) page[g] = at.page(a, 32 * jn + 16 * g);
@@ -607,19 +586,12 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
             wait_for<63, 0>();
             order();
         }
-        auto product = [&](auto first, auto count) {                     // tiles of 16 dims
-            constexpr int dt = decltype(first)::value, N = decltype(count)::value;
-            if constexpr (dt < DT) {
-                uint4_t v[N];
-                read_tr_all<N, 256 * (dt / FV), 16 * P::RS>(fv + dt % FV, v);
 #pragma unroll
-                for (int i = 0; i < N; ++i) O[dt + i] = mma16<BF>(v[i], Pr, O[dt + i]);
-            }
-        };
-        product(Num<0>{}, Num<4>{});
-        product(Num<4>{}, Num<DT == 6 ? 2 : 4>{});
-        product(Num<8>{}, Num<4>{});
-        product(Num<12>{}, Num<4>{});
+        for (int dt = 0; dt < DT; ++dt) {
+            const char* p = T + fv[dt % FV] + 256 * (dt / FV);
+            const uint2_t x = read_tr(p), y = read_tr(p + 16 * P::RS);
+            O[dt] = mma16<BF>(uint4_t{x[0], x[1], y[0], y[1]}, Pr, O[dt]);
+        }
         wait_for<63, 0>();                                               // the next values take the place of these
         order();
     }

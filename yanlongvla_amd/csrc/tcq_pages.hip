@@ -350,6 +350,7 @@ extern "C" int tcq_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int3
     const int e = book_of(a, table, lens, refs, free, lack, B, per_seq, pages, page_rows);
     if (e) return e;
     if (!src || !dst || n <= 0) return TCQ_ERR_ARG;
+    if (n > 65535) return TCQ_ERR_UNSUPPORTED;
     launch_k(k_pages_fork, dim3(n), dim3(256), 0, (hipStream_t)stream, a, src, dst, n);
     return launch_status();
 }
