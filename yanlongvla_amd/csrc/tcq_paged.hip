@@ -646,7 +646,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
 
 // The parts of a row joined: 64 threads for a row and head (4 dims each) and NG of them side by side over its parts, 4 / NG rows a workgroup; grid (rows,
 // B). Weights first (they are few), then the parts' outputs, eight loads under way.
-constexpr int MAX_PARTS = 64;        // one a lane
+constexpr int MAX_PARTS = 128;       // NP = 2 a lane
 template <bool BF, int NG>
 __global__ __launch_bounds__(256) void k_attend_join(Attn a) {
     __shared__ float4_t sums[4][64];
@@ -657,19 +657,29 @@ __global__ __launch_bounds__(256) void k_attend_join(Attn a) {
     const int64_t out = sq.c0 * Hq + (x < (int64_t)sq.n * Hq ? x : 0);
     const float* st = a.stat + out * a.S * 2;
     const float* p = a.part + out * a.S * a.D + 4 * d;
-    float mi = -__builtin_inff(), li = 0.f;                              // part d of the row's (at most 64)
-    if (d < a.S) {
-        const float2_t v = *gptr((const float2_t*)(st + 2 * d));
-        mi = v[0];
-        li = v[1];
+    constexpr int NP = NG == 1 ? 1 : MAX_PARTS / 64;                     // parts d, d + 64 of the row
+    float mi[NP], li[NP], M = -__builtin_inff(), L = 0.f;
+#pragma unroll
+    for (int r = 0; r < NP; ++r) {
+        const bool in = 64 * r + d < a.S;
+        const float2_t x = in ? *gptr((const float2_t*)(st + 2 * (64 * r + d))) : float2_t{-__builtin_inff(), 0.f};
+        mi[r] = x[0];
+        li[r] = x[1];
+        M = fmaxf(M, mi[r]);
     }
-    const float M = wave_max(mi), w = mi == -__builtin_inff() ? (M == mi ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mi - M), L = wave_sum(d < a.S ? w * li : 0.f);
+    M = wave_max(M);
     float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < NP; ++r) {
+        const float w = mi[r] == -__builtin_inff() ? (M == mi[r] ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mi[r] - M);
+        L = __builtin_fmaf(w, li[r], L);
 #pragma unroll 8
-    for (int i = g; i < a.S; i += NG) {
-        const float wi = lane_value(w, i);
-        if (on) v += *gptr((const float4_t*)(p + (int64_t)i * a.D)) * wi;
+        for (int i = g; i < min(64, a.S - 64 * r); i += NG) {
+            const float wi = lane_value(w, i);
+            if (on) v += *gptr((const float4_t*)(p + (int64_t)(64 * r + i) * a.D)) * wi;
+        }
     }
+    L = wave_sum(L);
     if constexpr (NG > 1) {
         sums[wave][d] = v;
         __syncthreads();
