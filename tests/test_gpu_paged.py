@@ -4,7 +4,7 @@ see nothing, rows of no sequence, keys and values that are not finite where no r
 replays.
 
 Tolerance of an output, elementwise: half a step of its type (eps / 2 relative), plus what the rounded probabilities and their sum change: each
-is off by at most d of itself (half a step of BF16, 2^-8; FP16 rounds towards zero, 2^-10), so a weight by 2 d and an output by 2 d sum p |v|. A score is a sum of
+is off by at most d of itself (half a step: BF16 2^-8, FP16 2^-11), so a weight by 2 d and an output by 2 d sum p |v|. A score is a sum of
 D products in FP32, off by at most e = D 2^-24 scale sum |q k|, and a weight with its sum by 2 e of itself; 1e-5 more for the exponentials
 (2^-22) and the sum of up to 64 terms a lane and tile."""
 import math
@@ -50,7 +50,7 @@ def formula(q, k, v, seen, scale=None):
 
 
 def close(got, o, a, e, dt):
-    d = 2.0 ** -8 if dt == BF else 2.0 ** -10
+    d = torch.finfo(dt).eps / 2
     nan = o.isnan()
     assert torch.equal(got.isnan(), nan)
     inf = o.isinf()

@@ -6,6 +6,14 @@
 // ones), are the right operand of O^T = V^T P^T where they are: the order in which the score product leaves the keys in a lane is the order in which
 // the values are fetched, by transposing reads of their rows in LDS. Rows of keys and values go from memory to LDS directly, in 16-byte
 // pieces whose place in the row is turned by the row's number so that the reads meet no bank twice.
+//
+// k_attend_rows, many rows: 32 rows a wave, so a wave reads every key and value of its tiles from LDS once for 32 rows: at 128 bytes a cycle that is as
+// long as its products (bound: LDS reads and vector instructions, 112 and 32 exponentials for 32 products a tile of 64 keys x 128 dims). 64
+// rows a wave would halve the reads, but leave one wave a SIMD (297 us for the case below at 235 to 250), eight waves a workgroup share the writes
+// only (242), and scores of the next tile computed beside the exponentials of this one gain nothing while the reads bound both (260). MI355X:
+// 2 x 4096 rows of 16 heads x 128 to 4096 and 3072 states 244 us (990 TFLOP/s; an 8192^3 product reaches 1260), 256 dims 1060, 64 dims 890.
+// k_attend_few, few rows: 16 rows a workgroup, four waves that share the keys; bound by memory from some MB on: 32 sequences of 16 heads on 8 x 128
+// behind 4 to 8 thousand keys 149 us (814 MB, 5.5 TB/s), by latencies below (one row behind 968 keys 10.1 us with the join).
 #include "tcq_device.h"
 #include "tcq_launch.h"
 
@@ -28,7 +36,7 @@ struct Attn {
     const char *k, *v;
     int64_t kb, kh, kt, vb, vh, vt;      // bytes: page (or sequence), head, token
     const int* table;                    // pages: (B, N)
-    const uint8_t* mask;                      // states: (B, T), mask_b apart
+    const uint8_t* mask;                 // states: (B, T), mask_b apart
     int64_t mask_b;
     const int *cu, *lens;
     u16* o;
@@ -48,8 +56,9 @@ __device__ __forceinline__ float4_t mma16(uint4_t a, uint4_t b, float4_t c) {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
-// two probabilities as 16-bit values, and their sum as the values say. FP16 rounds towards zero (one instruction): the sum
-// takes the same values, so the shift cancels and what remains is as large as that of the nearest ones.
+// two probabilities as 16-bit values, to nearest, and their sum as the values say: the weights that the values get add up to one. (16 bits are what the
+// products take; a second product for the rest would double theirs. Relative error of an output against 64 bits 2.1e-3 in BF16, 2.8e-4
+// in FP16, where its own rounding is 1.7e-3 and 2.1e-4.)
 template <bool BF>
 __device__ __forceinline__ u32 prob2(float a, float b) {
     return BF ? bf16_cvt2(a, b) : __builtin_bit_cast(u32, __builtin_convertvector(float2_t{a, b}, half2_t));
@@ -644,15 +653,16 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     }
 }
 
-// The parts of a row joined: 64 threads for a row and head (4 dims each) and NG of them side by side over its parts, 4 / NG rows a workgroup; grid (rows,
-// B). Weights first (they are few), then the parts' outputs, eight loads under way.
+// The parts of a row joined: 64 threads for a row and head (4 dims each) and NG of them side by side over its parts, in workgroups of four waves or more; grid
+// (rows, B). Weights first (they are few), then the parts' outputs, eight loads under way. (16 rows of 128 parts: 13 us with NG = 4.)
 constexpr int MAX_PARTS = 128;       // NP = 2 a lane
 template <bool BF, int NG>
-__global__ __launch_bounds__(256) void k_attend_join(Attn a) {
-    __shared__ float4_t sums[4][64];
+__global__ __launch_bounds__(64 * (NG > 4 ? NG : 4)) void k_attend_join(Attn a) {
+    constexpr int NW = NG > 4 ? NG : 4;
+    __shared__ float4_t sums[NW][64];
     const Seq sq = seq_of(a, blockIdx.y);
     const int Hq = a.Hk * a.G, d = threadIdx.x & 63, wave = threadIdx.x >> 6, g = wave % NG;
-    const int64_t x = (int64_t)blockIdx.x * (4 / NG) + wave / NG;
+    const int64_t x = (int64_t)blockIdx.x * (NW / NG) + wave / NG;
     const bool on = x < (int64_t)sq.n * Hq && 4 * d < a.D;
     const int64_t out = sq.c0 * Hq + (x < (int64_t)sq.n * Hq ? x : 0);
     const float* st = a.stat + out * a.S * 2;
@@ -697,7 +707,7 @@ __global__ __launch_bounds__(256) void k_attend_join(Attn a) {
 //   over at most 16 tiles: their four waves share the keys of a row, where the other kernel would need parts and their join (50 rows of 32 heads x 48 to
 //   600 keys 6.6 us against 10.0, 300 x 300 of 16 x 64 7.1 against 10.4, 8 x 50 rows of 8 heads on 1 x 256 behind 850 22.9 against 27.4; 4000 keys 83
 //   against 46).
-//   Parts: as many as fill the chip, of one tile (the other kernel: two) or more. Few rows take 1024 workgroups (32 sequences of 16 heads on 8 x 128 behind
+//   Parts: as many as fill the chip (at most 128), of one tile (the other kernel: two) or more. Few rows take 1024 workgroups (32 sequences of 16 heads on 8 x 128 behind
 //   4 to 8 thousand keys 176 us, 512: 203, 2048: 179), but 16 and more rows a workgroup, whose parts are larger to write and to join, 512 over many
 //   tiles (4 x 16 rows behind 8000 keys 42.6, 1024: 53) and 256 over few. No parts where they save less than their join takes, about 4 us, at
 //   D / 200 us a tile.
@@ -762,11 +772,13 @@ int run(Attn& a, bool bf, bool paged, int B, int keys, float* part, hipStream_t 
     const int64_t rows = (int64_t)a.most * Hq;
 #define JOIN(NG)                                                                                                        \
     do {                                                                                                                \
-        const dim3 grid((u32)((rows + 4 / NG - 1) / (4 / NG)), B);                                                      \
-        if (bf) launch_k(k_attend_join<true, NG>, grid, dim3(256), 0, st, a);                                           \
-        else launch_k(k_attend_join<false, NG>, grid, dim3(256), 0, st, a);                                             \
+        constexpr int NW = NG > 4 ? NG : 4;                                                                             \
+        const dim3 grid((u32)((rows + NW / NG - 1) / (NW / NG)), B);                                                    \
+        if (bf) launch_k(k_attend_join<true, NG>, grid, dim3(64 * NW), 0, st, a);                                       \
+        else launch_k(k_attend_join<false, NG>, grid, dim3(64 * NW), 0, st, a);                                         \
     } while (0)
-    if (a.S > 8) JOIN(4);
+    if (a.S > 32) JOIN(16);
+    else if (a.S > 8) JOIN(4);
     else JOIN(1);
 #undef JOIN
     return launch_status();
