@@ -11,7 +11,7 @@
 // long as its products (bound: LDS reads and vector instructions, 112 and 32 exponentials for 32 products a tile of 64 keys x 128 dims). 64
 // rows a wave would halve the reads, but leave one wave a SIMD (297 us for the case below at 235 to 250), eight waves a workgroup share the writes
 // only (242), and scores of the next tile computed beside the exponentials of this one gain nothing while the reads bound both (260). MI355X:
-// 2 x 4096 rows of 16 heads x 128 to 4096 and 3072 states 244 us (990 TFLOP/s; an 8192^3 product reaches 1260), 256 dims 1060, 64 dims 890.
+// 2 x 4096 rows of 16 heads x 128 to up to 4096 states 240 us (1000 TFLOP/s; an 8192^3 product reaches 1260), 256 dims 1060, 64 dims 890.
 // k_attend_few, few rows: 16 rows a workgroup, four waves that share the keys; bound by memory from some MB on: 32 sequences of 16 heads on 8 x 128
 // behind 4 to 8 thousand keys 149 us (814 MB, 5.5 TB/s), by latencies below (one row behind 968 keys 10.1 us with the join).
 #include "tcq_device.h"
