@@ -389,3 +389,63 @@ def test_cross_ragged_queries_views_and_replays():
             g.replay()
         for g, out in graphs:
             assert torch.equal(out[:sum(new)], want[:sum(new)])
+
+
+# ------------------------------------------------------------------------------------------------------- many workgroups, shared pages
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('B', [9, 64, 70])
+def test_more_tiles_than_fit_at_once(B, causal):
+    """Calls of more than 512 workgroups, which are ordered by the keys that they see (up to 64 sequences): lengths of all kinds, sequences without rows,
+    rows that see nothing."""
+    from yanlongvla_amd import kernels as K
+    Hq, H, D, T, dt = 16, 8, 64, 16, BF
+    gen = torch.Generator().manual_seed(B)
+    new = [0 if b % 7 == 3 else int(torch.randint(1, 700 if B < 64 else 150, (1,), generator=gen)) for b in range(B)]
+    lens = [max(1, n - 40) if b % 5 == 1 else n + int(torch.randint(0, 200, (1,), generator=gen)) for b, n in enumerate(new)]
+    pool = Pool(lens, H, D, T, dt, seed=B)
+    q = rand(sum(new) + 2, Hq, D, seed=7, dt=dt, by=2.0)
+    cu = ints([sum(new[:b]) for b in range(B + 1)])
+    o = torch.full_like(q, 7.0)
+    K.paged_attend(q, pool.pages, pool.table, pool.lens, o=o, causal=causal, cu=cu, most=700)
+    assert (o[sum(new):] == 7).all()
+    check(o, q, pool, lens, new, causal, dt)
+
+
+def test_cross_attention_of_many_tiles():
+    from yanlongvla_amd import kernels as K
+    B, M, T, Hq, H, D = 5, 900, 150, 16, 16, 72
+    k, v, q = rand(B, T, H, D, seed=1), rand(B, T, H, D, seed=2), rand(B * M, Hq, D, seed=3)
+    lens = ints([150, 0, 77, 1, 128])
+    cross_check(K.cross_attend(q, k, v, lens), q, k, v, lens, None, M, BF)
+    mask = torch.rand(B, T, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV) < 0.5
+    cross_check(K.cross_attend(q, k, v, lens, mask), q, k, v, lens, mask, M, BF)
+
+
+def test_forks_attend_to_shared_pages_and_outputs_in_place():
+    """Sequences that share pages give the same rows; an output may be the queries' own tensor; calls on two streams at once."""
+    from yanlongvla_amd import kernels as K
+    H, Hq, D, T, n = 2, 4, 128, 32, 3000
+    pool, pt = K.kv_pages(110, H, D, DEV, T), K.page_table(3, 100, 110, DEV, T)
+    k, v = rand(n, H, D, seed=1), rand(n, H, D, seed=2)
+    start = K.pages_take(pt, pool, ints([n, 0, 0]))
+    K.paged_append(pool, k, v, pt.table, pt.lens, start, ints([0, n, n, n]), n)
+    K.pages_fork(pt, ints([0, 0]), ints([1, 2]))
+    for m in (1, 40, 200):
+        one = rand(m, Hq, D, seed=m)
+        q = one.repeat(3, 1, 1)
+        got = K.paged_attend(q, pool, pt.table, pt.lens)
+        assert torch.equal(got[:m], got[m:2 * m]) and torch.equal(got[:m], got[2 * m:])
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        outs = []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs.append([K.paged_attend(q, pool, pt.table, pt.lens) for _ in range(5)])
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(x, got) for x in outs[0] + outs[1])
+        mine = q.clone()
+        K.paged_attend(mine, pool, pt.table, pt.lens, o=mine)
+        assert torch.equal(mine, got)
+        wide = one[:1].expand(m, Hq, D)                                        # the same query in every row
+        assert torch.equal(K.paged_attend(wide, pool, pt.table[:1], pt.lens[:1], causal=False)[0], K.paged_attend(wide.contiguous(), pool, pt.table[:1], pt.lens[:1], causal=False)[m - 1])
