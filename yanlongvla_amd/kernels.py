@@ -752,7 +752,7 @@ def _queries(what, q, Hk, D, dt, o):
 
 def paged_attend(q, pages, table, lens, o=None, causal=True, cu=None, most=None, scale=None, keys=None):
     """Attention of q (rows, Hq, D; the pages' type, 16-byte aligned, strides multiples of 8) over the first lens[b] rows of every sequence in the
-    pages (one layer's, any strides that are multiples of 8) that table (B, N) names, Hq a multiple of their heads: o (rows, Hq, D). B equal
+    pages (one layer's, any strides that are multiples of 8, a token's of at least D) that table (B, N) names, Hq a multiple of their heads: o (rows, Hq, D). B equal
     shares of the rows, or cu and most as in paged_append; causal, scale, keys and rows of no sequence as in kv8_attend."""
     ps, pk, pv, dt = _one_layer(pages, 'paged_attend')
     B, N = _tables('paged_attend', table, lens)
@@ -790,7 +790,7 @@ class PagedRows:
 
 def cross_attend(q, k, v, lens=None, mask=None, o=None, cu=None, most=None, scale=None):
     """Attention of q (rows, Hq, D; BF16 / FP16, 16-byte aligned, strides multiples of 8) to an encoder's states of another length: k, v (B, T, H, D) of the
-    same type, 16-byte aligned, strides multiples of 8 (views into a product's rows), Hq a multiple of H. Every row of sequence b sees
+    same type, 16-byte aligned, strides multiples of 8, a token's of at least D (views into a product's rows), Hq a multiple of H. Every row of sequence b sees
     keys 0 .. lens[b] - 1 (B, int32, on the device; None: all) with mask[b, j] (B, T, bool; None: all): o (rows, Hq, D), zeros where
     that is none. B equal shares of the rows, or cu and most as in kv8_attend; scale: of the scores, 1 / sqrt(D) by default."""
     ks, sk, sv, dt = k.shape, k.stride(), v.stride(), k.dtype
