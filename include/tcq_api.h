@@ -607,7 +607,8 @@ int tcq_gemmf_tcq_hT(const void* bits, const int8_t* t8, const void* hT, int ldh
  * tcq_pages_copy: page src[i] to page dst[i] in all layers, n pairs; pairs outside the pool are left out, no page may be a dst twice, or a dst and a
  *   src. The bookkeeping is not told.
  * tcq_paged_append: rows k, v (any strides in elements) to positions start[b] + i of their sequence: B equal shares of `most` rows, or rows cu[b] ..
- *   cu[b + 1] - 1, at most `most` of them. Rows at or past lens[b], and those whose entry names no page, are dropped. */
+ *   cu[b + 1] - 1, at most `most` of them. Rows at or past lens[b], and those whose entry names no page, are dropped. The
+ *   pages that rows from the last take's start on go to are the sequence's own; others, and those forked since, change for all that hold them. */
 int tcq_pages_take(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows,
                    const int32_t* take, int32_t* start, void* k, void* v, int layers, int64_t page_bytes, int32_t* moves, tcq_stream_t stream);
 int tcq_pages_fork(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows,
