@@ -16,6 +16,7 @@
 // behind 4 to 8 thousand keys 149 us (814 MB, 5.5 TB/s), by latencies below (one row behind 968 keys 10.1 us with the join).
 #include "tcq_device.h"
 #include "tcq_launch.h"
+#include "tcq_paged_rows.h"
 
 #include <type_traits>
 
@@ -662,9 +663,10 @@ __global__ __launch_bounds__(64 * (NG > 4 ? NG : 4)) void k_attend_join(Attn a) 
     __shared__ float4_t sums[NW][64];
     const Seq sq = seq_of(a, blockIdx.y);
     const int Hq = a.Hk * a.G, d = threadIdx.x & 63, wave = threadIdx.x >> 6, g = wave % NG;
-    const int64_t x = (int64_t)blockIdx.x * (NW / NG) + wave / NG;
-    const bool on = x < (int64_t)sq.n * Hq && 4 * d < a.D;
-    const int64_t out = sq.c0 * Hq + (x < (int64_t)sq.n * Hq ? x : 0);
+    static_assert(NG == 1 || NG == NW, "the waves that meet at the barrier have one row: they leave together");
+    const int64_t out = join_row(sq.c0, sq.n, Hq, (int64_t)blockIdx.x * (NW / NG) + wave / NG);
+    if (out < 0) return;                                                 // (before the loads: behind the rows the workspace ends)
+    const bool on = 4 * d < a.D;
     const float* st = a.stat + out * a.S * 2;
     const float* p = a.part + out * a.S * a.D + 4 * d;
     constexpr int NP = NG == 1 ? 1 : MAX_PARTS / 64;                     // parts d, d + 64 of the row
