@@ -29,7 +29,9 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 // FP16 probabilities lie 2^7 higher (the maximum follows in steps of 2^8, so at most 2^15): those of 2^-21 of the largest keep all their digits
 template <bool BF> constexpr float LIFT = BF ? 0.f : 7.f;
-constexpr float LOWEST = -3.0e38f;       // the maximum of a row that has seen keys, all of them with scores of -inf
+// The maximum of a row that has seen keys, all of them with scores of -inf. Maxima are of the products q k: times a scale above 0.78 it would be the
+// -inf of a row that has seen none.
+constexpr float LOWEST = -3.0e38f;
 
 struct Attn {
     const u16* q;
@@ -41,7 +43,7 @@ struct Attn {
     int64_t mask_b;
     const int *cu, *lens;
     u16* o;
-    float *part, *stat;                  // split: outputs (row, head, split, D) and maxima / sums (.., 2)
+    float *part, *stat;                  // split: outputs (row, head, split, D) and maxima (of the products, not scaled) / sums (.., 2)
     int rows, most, Hk, G, D, N, shift, pages, cap, causal, S, tiles, sorted;
     float sl;
 };
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
                 const int d = 32 * dt + 8 * e + 4 * h2;
                 if (d < a.D) *gptr((float4_t*)(p + d)) = float4_t{O[dt][4 * e], O[dt][4 * e + 1], O[dt][4 * e + 2], O[dt][4 * e + 3]};
             }
-        if (h2 == 0) *gptr((float2_t*)(a.stat + (out * a.S + s) * 2)) = float2_t{m * a.sl, l};
+        if (h2 == 0) *gptr((float2_t*)(a.stat + (out * a.S + s) * 2)) = float2_t{m, l};
         return;
     }
     const float inv = m == -__builtin_inff() && l == 0.f ? 0.f : 1.f / l;
@@ -625,7 +627,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     float* const Y = X + W * 16 * OS;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) *(float4_t*)(X + (wave * 16 + lr) * OS + 16 * dt + 4 * lg) = O[dt];
-    if (lg == 0) *(float2_t*)(Y + (wave * 16 + lr) * 2) = float2_t{m * a.sl, l};
+    if (lg == 0) *(float2_t*)(Y + (wave * 16 + lr) * 2) = float2_t{m, l};
     __syncthreads();
     const int D4 = a.D >> 2;
     for (int u = threadIdx.x; u < 16 * D4; u += 64 * W) {
@@ -638,7 +640,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
         float4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float mw = Y[(w * 16 + r) * 2], x = mw == -__builtin_inff() ? (M == mw ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mw - M);
+            const float mw = Y[(w * 16 + r) * 2], x = mw == -__builtin_inff() ? (M == mw ? 1.f : 0.f) : __builtin_amdgcn_exp2f((mw - M) * a.sl);
             L = __builtin_fmaf(x, Y[(w * 16 + r) * 2 + 1], L);
             v += *(const float4_t*)(X + (w * 16 + r) * OS + d) * x;
         }
@@ -683,7 +685,7 @@ __global__ __launch_bounds__(64 * (NG > 4 ? NG : 4)) void k_attend_join(Attn a) 
     float4_t v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < NP; ++r) {
-        const float w = mi[r] == -__builtin_inff() ? (M == mi[r] ? 1.f : 0.f) : __builtin_amdgcn_exp2f(mi[r] - M);
+        const float w = mi[r] == -__builtin_inff() ? (M == mi[r] ? 1.f : 0.f) : __builtin_amdgcn_exp2f((mi[r] - M) * a.sl);
         L = __builtin_fmaf(w, li[r], L);
 #pragma unroll 8
         for (int i = g; i < min(64, a.S - 64 * r); i += NG) {
