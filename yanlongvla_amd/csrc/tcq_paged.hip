@@ -27,6 +27,9 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
+// A probability is exp2((S - m) sl + LIFT), the difference first: S sl - m sl as one multiply-add with a rounded m sl is off by up to 2^-25 |m sl|, which
+// from scores of about 10^7 on takes FP16 probabilities (10^9: BF16) out of their range and gives keys met before and after a new maximum different
+// weights. The maximum follows for the same reason when S - m passes its step, not when S passes a rounded m + step.
 // FP16 probabilities lie 2^7 higher (the maximum follows in steps of 2^8, so at most 2^15): those of 2^-21 of the largest keep all their digits
 template <bool BF> constexpr float LIFT = BF ? 0.f : 7.f;
 // The maximum of a row that has seen keys, all of them with scores of -inf. Maxima are of the products q k: times a scale above 0.78 it would be the
@@ -58,6 +61,10 @@ template <bool BF>
 __device__ __forceinline__ float4_t mma16(uint4_t a, uint4_t b, float4_t c) {
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ float prob(float d, float sl) {
+    return __builtin_amdgcn_exp2f(BF ? d * sl : __builtin_fmaf(d, sl, LIFT<BF>));
 }
 // two probabilities as 16-bit values, to nearest, and their sum as the values say: the weights that the values get add up to one. (16 bits are what the
 // products take; a second product for the rest would double theirs. Relative error of an output against 64 bits 2.1e-3 in BF16, 2.8e-4
@@ -321,7 +328,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
         for (int e = 0; e < 16; ++e) O[dt][e] = 0.f;
     float m = -__builtin_inff(), l = 0.f;
     u32 odd = 0;
-    const float thr = 8.f / a.sl;
+    const float thr = fminf(8.f / a.sl, __FLT_MAX__);                    // (a first maximum passes it whatever the scale)
 
     int page[U], mb = 0;                                                 // pages of the next tile
     u64 b0 = 0, b1 = 0;                                                  // MASK: bits of tiles j, j + 1
@@ -378,7 +385,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, S[kt][e]);
         mx = fmaxf(mx, lane_xor(mx, 32, lane));
-        const bool up = mx > m + thr;                                    // the maximum follows in steps: probabilities stay below 2^8
+        const bool up = mx - m > thr;                                    // the maximum follows in steps: probabilities stay below 2^8
         if (__builtin_amdgcn_ballot_w64(up)) {                           // uniform
             const float al = up ? __builtin_amdgcn_exp2f((m - mx) * a.sl) : 1.f;
             l *= al;
@@ -386,13 +393,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
             for (int dt = 0; dt < DT; ++dt) O[dt] *= al;
             m = up ? mx : m;
         }
-        const float mc = fmaxf(m * a.sl, -__FLT_MAX__) - LIFT<BF>;       // (a row that has seen nothing yet: its scores are -inf)
+        const float mr = fmaxf(m, LOWEST);                               // (a row that has seen nothing yet: its scores are -inf)
         uint4_t Pr[2 * NK];
 #pragma unroll
         for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const u32 x = prob2<BF>(__builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][e], a.sl, -mc)), __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][e + 1], a.sl, -mc)));
+                const u32 x = prob2<BF>(prob<BF>(S[kt][e] - mr, a.sl), prob<BF>(S[kt][e + 1] - mr, a.sl));
                 l = sum2<BF>(x, l);
                 Pr[2 * kt + (e >> 3)][(e >> 1) & 3] = x;
             }
@@ -534,7 +541,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     for (int dt = 0; dt < DT; ++dt) O[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
     float m = -__builtin_inff(), l = 0.f;
     u32 odd = 0;
-    const float thr = 8.f / a.sl;
+    const float thr = fminf(8.f / a.sl, __FLT_MAX__);                    // (a first maximum passes it whatever the scale)
     int j = t0 + wave, page[2];
     u32 bits = bits_of(j);
 #pragma unroll
@@ -574,7 +581,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
             for (int e = 0; e < 4; ++e) mx = fmaxf(mx, S[g][e]);
         mx = fmaxf(mx, lane_xor(mx, 16, lane));
         mx = fmaxf(mx, lane_xor(mx, 32, lane));
-        const bool up = mx > m + thr;
+        const bool up = mx - m > thr;
         if (__builtin_amdgcn_ballot_w64(up)) {
             const float al = up ? __builtin_amdgcn_exp2f((m - mx) * a.sl) : 1.f;
             l *= al;
@@ -582,12 +589,11 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
             for (int dt = 0; dt < DT; ++dt) O[dt] *= al;
             m = up ? mx : m;
         }
-        const float mc = fmaxf(m * a.sl, -__FLT_MAX__) - LIFT<BF>;
+        const float mr = fmaxf(m, LOWEST);
         uint4_t Pr;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            Pr[x] = prob2<BF>(__builtin_amdgcn_exp2f(__builtin_fmaf(S[x >> 1][2 * (x & 1)], a.sl, -mc)),
-                              __builtin_amdgcn_exp2f(__builtin_fmaf(S[x >> 1][2 * (x & 1) + 1], a.sl, -mc)));
+            Pr[x] = prob2<BF>(prob<BF>(S[x >> 1][2 * (x & 1)] - mr, a.sl), prob<BF>(S[x >> 1][2 * (x & 1) + 1] - mr, a.sl));
             l = sum2<BF>(Pr[x], l);
         }
         wait_for<2 * KS, 15>();                                          // the values are there; the next keys may be under way
@@ -788,6 +794,9 @@ int run(Attn& a, bool bf, bool paged, int B, int keys, float* part, hipStream_t 
     return launch_status();
 }
 
+// The scale to powers of two: above 0 and finite, so that 0 * -inf and 0 * inf do not come up (scores times 2^-149 are all 0)
+float log2_scale(float s) { return fminf(fmaxf(s * 1.44269504088896341f, 0x1p-149f), __FLT_MAX__); }
+
 constexpr int64_t MANY = 0x7fffffff;
 // what both attentions ask of their arguments
 int refuse(const void* q, int64_t q_tok, int64_t q_head, int dtype, const int32_t* cu, int rows, int most, int B, int Hq, int Hk, int D, const void* k,
@@ -823,7 +832,7 @@ extern "C" int tcq_paged_attend(const void* q, int64_t q_tok, int64_t q_head, in
     a.table = table, a.cu = cu, a.lens = lens, a.o = (u16*)o;
     a.rows = rows, a.most = most, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.N = per_seq, a.shift = 31 - __builtin_clz(page_rows), a.pages = pages;
     a.cap = page_rows * per_seq, a.causal = causal != 0;
-    a.sl = fmaxf(score_scale * 1.44269504088896341f, 1e-30f);
+    a.sl = log2_scale(score_scale);
     return run(a, dtype == TCQ_BF16, true, B, min(keys, a.cap), part, (hipStream_t)stream);
 }
 
@@ -843,6 +852,6 @@ extern "C" int tcq_cross_attend(const void* q, int64_t q_tok, int64_t q_head, in
     a.kb = 2 * k_seq, a.kh = 2 * k_head, a.kt = 2 * k_tok, a.vb = 2 * v_seq, a.vh = 2 * v_head, a.vt = 2 * v_tok;
     a.mask = mask, a.mask_b = mask_seq, a.cu = cu, a.lens = lens, a.o = (u16*)o;
     a.rows = rows, a.most = most, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.cap = keys;
-    a.sl = fmaxf(score_scale * 1.44269504088896341f, 1e-30f);
+    a.sl = log2_scale(score_scale);
     return run(a, dtype == TCQ_BF16, false, B, keys, part, (hipStream_t)stream);
 }
