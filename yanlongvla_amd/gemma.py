@@ -226,6 +226,8 @@ class PagedKVCache:
 
     def _only(self, sequence, n):
         """take and cu of n rows of one sequence and none of the others."""
+        if not 0 <= sequence < self.sequences:
+            raise IndexError(f'PagedKVCache: sequence {sequence} of {self.sequences}')
         take = torch.zeros_like(self.active)
         take[sequence:sequence + 1].fill_(n)
         cu = torch.zeros(self.sequences + 1, dtype=torch.int32, device=take.device)
@@ -233,7 +235,7 @@ class PagedKVCache:
         return take, cu
 
     def extend(self, ks, vs, sequence):
-        """Rows ks[i], vs[i] (n, heads * D) of every layer i behind those of one sequence, as a prefill returns them."""
+        """Rows ks[i], vs[i] (n, heads * D) of every layer i behind those of one sequence (0 .. sequences - 1), as a prefill returns them."""
         from . import kernels
         n, D = ks[0].shape[0], self.pool.k.shape[-1]
         take, cu = self._only(sequence, n)
