@@ -705,6 +705,17 @@ def _one_layer(pages, what):
     return s, sk, sv, k.dtype
 
 
+def _rows_apart(size, stride):
+    """Whether the rows of pages (.., D) with these strides are different ones, each axis stepping over all that the shorter steps span."""
+    span = size[-1]
+    for step, n in sorted(zip(stride[:-1], size[:-1])):
+        if n > 1:
+            if step < span:
+                return False
+            span += (n - 1) * step
+    return True
+
+
 def _tables(what, table, lens):
     if not (len(table.shape) == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.shape[0] > 0 and table.shape[1] > 0):
         raise ValueError(f'{what}: table must be a contiguous int32 (sequences, pages of one)')
@@ -726,9 +737,8 @@ def paged_append(pages, k, v, table, lens, start, cu=None, most=None):
     _counts('paged_append', start, B)
     rows = size[0]
     most = _most('paged_append', rows, B, cu, most)
-    for t in (pk, pv):
-        if (ps[0] > 1 and t[0] == 0) or (ps[1] > 1 and t[1] == 0) or t[2] == 0:
-            raise ValueError('paged_append: rows of the pages overlap (an expanded tensor)')
+    if not all(t.is_contiguous() or _rows_apart(ps, t.stride()) for t in pages) or pages[0].data_ptr() == pages[1].data_ptr():
+        raise ValueError('paged_append: rows of the pages overlap (an expanded tensor, windows, or keys and values in one place)')
     xk, xv, xt, xl, xs, xc, xpk, xpv = _ptrs('paged_append', k, v, table, lens, start, cu, *pages)
     if most and rows:
         rc = _lib.lib().tcq_paged_append(xk, sk[0], sk[1], xv, sv[0], sv[1], xc, rows, most, B, ps[1], ps[3], xpk, pk[0], pk[1], pk[2], xpv, pv[0], pv[1],
