@@ -1,8 +1,8 @@
-"""CPU test of what a cache in pages refuses before it takes a page: sequences that it does not have."""
+"""CPU tests of what a cache in pages refuses before it takes a page: sequences that it does not have, a start that is another operand."""
 import pytest
 import torch
 
-from yanlongvla_amd import gemma
+from yanlongvla_amd import gemma, kernels
 from yanlongvla_amd._lib import TcqError
 
 
@@ -18,3 +18,14 @@ def test_sequences_that_are_not_there(sequence):
     for there in (0, 2):
         with pytest.raises(TcqError):                                        # host tensors
             cache.extend(rows, rows, there)
+
+
+def test_a_start_of_its_own():
+    """Where it is take the rows to take would be gone after the call, and a replay take as many as there are."""
+    pt, pool = kernels.page_table(2, 4, 8, 'cpu', 16), kernels.kv_pages(8, 1, 64, 'cpu', 16)
+    take = torch.ones(2, dtype=torch.int32)
+    for start in (take, take.view(2), pt.lens):
+        with pytest.raises(ValueError, match='of its own'):
+            kernels.pages_take(pt, pool, take, start)
+    with pytest.raises(TcqError):                                            # host tensors
+        kernels.pages_take(pt, pool, take, torch.zeros_like(take))

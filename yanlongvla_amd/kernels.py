@@ -635,8 +635,8 @@ def pages_take(pt, pages, take, start=None):
         start = torch.empty_like(take)
     else:
         _counts('pages_take', start, B)
-        if start.data_ptr() == pt.lens.data_ptr():
-            raise ValueError('pages_take: start must be a tensor of its own')
+        if start.data_ptr() in (pt.lens.data_ptr(), take.data_ptr()):
+            raise ValueError('pages_take: start must be a tensor of its own, not lens or take')
     *book, tk, ts, pk, pv = _ptrs('pages_take', *pt[:5], take, start, *pages)
     moves = torch.empty(2 * B + 1, dtype=torch.int32, device=take.device)
     rc = _lib.lib().tcq_pages_take(*book, *size, tk, ts, pk, pv, *pool, moves.data_ptr(), stream())
