@@ -1,4 +1,5 @@
-"""CPU tests of what a cache in pages refuses before it takes a page: sequences that it does not have, a start that is another operand."""
+"""CPU tests of what a cache in pages refuses before it takes a page: sequences that it does not have, a start that
+is another operand, rows of other layers or sizes."""
 import pytest
 import torch
 
@@ -29,3 +30,18 @@ def test_a_start_of_its_own():
             kernels.pages_take(pt, pool, take, start)
     with pytest.raises(TcqError):                                            # host tensors
         kernels.pages_take(pt, pool, take, torch.zeros_like(take))
+
+
+def test_rows_of_other_layers_or_sizes():
+    cache = gemma.PagedKVCache(2, 3, 8, 64, 'cpu', rows=16, heads=2)
+    one = torch.zeros(5, 128, dtype=torch.bfloat16)
+    good = [one, one]
+    for bad in ([], [one], [one] * 3, [one, one[:4]], [one, one[:, :64]], [one, one.half()], [one, one.float()]):
+        for ks, vs in ((bad, bad), (good, bad), (bad, good)):
+            with pytest.raises(ValueError):
+                cache.extend(ks, vs, 0)
+    with pytest.raises(TcqError):                                            # host tensors
+        cache.extend(good, good, 0)
+    model = gemma.BackbonePolicy(layers=3, width=64, hidden=64, heads=1, head_dim=64, vocab=8)
+    with pytest.raises(ValueError):
+        model.prefill_chunk(torch.zeros(5, 64), cache, 0)

@@ -237,7 +237,10 @@ class PagedKVCache:
     def extend(self, ks, vs, sequence):
         """Rows ks[i], vs[i] (n, heads * D) of every layer i behind those of one sequence (0 .. sequences - 1), as a prefill returns them."""
         from . import kernels
-        n, D = ks[0].shape[0], self.pool.k.shape[-1]
+        L, H, D, dt = len(self.layers), self.pool.k.shape[2], self.pool.k.shape[4], self.pool.k.dtype
+        n = ks[0].shape[0] if len(ks) else 0
+        if not len(ks) == len(vs) == L or any(t.shape[0] != n or t.numel() != n * H * D or t.dtype != dt for t in (*ks, *vs)):
+            raise ValueError(f'PagedKVCache.extend: keys and values of {L} layers, each (rows, {H * D}) {dt}')
         take, cu = self._only(sequence, n)
         start = kernels.pages_take(self.table, self.pool, take)
         for layer, k, v in zip(self.layers, ks, vs):
@@ -355,6 +358,8 @@ class BackbonePolicy(nn.Module):
     def prefill_chunk(self, x, cache, sequence):
         """x (n, width), the next part of a sequence's prefix, behind the rows that a PagedKVCache holds of it: the hidden states, with the rows written
         into the cache. Parts of any length give the rows of one prefill."""
+        if len(cache.layers) != len(self.stack.layers):
+            raise ValueError(f'prefill_chunk: a cache of {len(cache.layers)} layers for {len(self.stack.layers)}')
         h = x
         for layer, rows in zip(self.stack.layers, cache.chunk(sequence, x.shape[0])):
             h, _, _ = layer(h, rows, None, causal_offset=0)
