@@ -188,8 +188,6 @@ __device__ __forceinline__ void row_to_lds(const char* base, u32 bytes, u32 off,
 
 __device__ __forceinline__ u64 first_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
-template <int N> using Num = std::integral_constant<int, N>;
-
 // Which tile of R rows of which sequence and head workgroup k takes: the k-th when they are ordered by the keys that they see (in steps of 64), the
 // most first, so that the last ones to start are short. A lane counts for one sequence (at most 64); found by bisection of the number of keys.
 struct Job {

@@ -78,7 +78,7 @@ class GemmaAttention(nn.Module):
         """Attention of the projected q / k / v (the cache rows, if any, before this call's own keys / values). Device
         BF16 tensors go to the HIP attention kernel; host tensors (CPU twins in tests) to the same formula in PyTorch. cache_k may
         be a kernels.KV8Rows: the rows (at most 64) then go into that 8-bit cache (causal_offset: its length, or None for every row to see
-        all), or a kernels.PagedRows: equal shares of the rows go to the sequences of its table."""
+        all), or a kernels.PagedRows: the rows go to the sequences of its table, equal shares or as its cu says."""
         if hasattr(cache_k, 'core'):
             return cache_k.core(q, k, v, self.heads, causal_offset is not None)
         if self._device(q):
