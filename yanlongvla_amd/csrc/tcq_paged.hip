@@ -48,7 +48,7 @@ struct Attn {
     u16* o;
     float *part, *stat;                  // split: outputs (row, head, split, D) and maxima (of the products, not scaled) / sums (.., 2)
     int rows, most, Hk, G, D, N, shift, pages, cap, causal, S, tiles, sorted;
-    float sl;
+    float sl, step;                      // the scale to powers of two, and how far scores may pass the maximum before it follows: 2^8
 };
 
 
@@ -326,7 +326,6 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
         for (int e = 0; e < 16; ++e) O[dt][e] = 0.f;
     float m = -__builtin_inff(), l = 0.f;
     u32 odd = 0;
-    const float thr = fminf(8.f / a.sl, __FLT_MAX__);                    // (a first maximum passes it whatever the scale)
 
     int page[U], mb = 0;                                                 // pages of the next tile
     u64 b0 = 0, b1 = 0;                                                  // MASK: bits of tiles j, j + 1
@@ -383,7 +382,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attend_rows(Attn a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, S[kt][e]);
         mx = fmaxf(mx, lane_xor(mx, 32, lane));
-        const bool up = mx - m > thr;                                    // the maximum follows in steps: probabilities stay below 2^8
+        const bool up = mx - m > a.step;                                    // the maximum follows in steps: probabilities stay below 2^8
         if (__builtin_amdgcn_ballot_w64(up)) {                           // uniform
             const float al = up ? __builtin_amdgcn_exp2f((m - mx) * a.sl) : 1.f;
             l *= al;
@@ -539,7 +538,6 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
     for (int dt = 0; dt < DT; ++dt) O[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
     float m = -__builtin_inff(), l = 0.f;
     u32 odd = 0;
-    const float thr = fminf(8.f / a.sl, __FLT_MAX__);                    // (a first maximum passes it whatever the scale)
     int j = t0 + wave, page[2];
     u32 bits = bits_of(j);
 #pragma unroll
@@ -579,7 +577,7 @@ __global__ __launch_bounds__(64 * W, DP == 256 ? 2 : 4) void k_attend_few(Attn a
             for (int e = 0; e < 4; ++e) mx = fmaxf(mx, S[g][e]);
         mx = fmaxf(mx, lane_xor(mx, 16, lane));
         mx = fmaxf(mx, lane_xor(mx, 32, lane));
-        const bool up = mx - m > thr;
+        const bool up = mx - m > a.step;
         if (__builtin_amdgcn_ballot_w64(up)) {
             const float al = up ? __builtin_amdgcn_exp2f((m - mx) * a.sl) : 1.f;
             l *= al;
@@ -792,8 +790,12 @@ int run(Attn& a, bool bf, bool paged, int B, int keys, float* part, hipStream_t 
     return launch_status();
 }
 
-// The scale to powers of two: above 0 and finite, so that 0 * -inf and 0 * inf do not come up (scores times 2^-149 are all 0)
-float log2_scale(float s) { return fminf(fmaxf(s * 1.44269504088896341f, 0x1p-149f), __FLT_MAX__); }
+// The scale is above 0 and finite, so that 0 * -inf and 0 * inf do not come up (scores times 2^-149 are all 0); a first maximum passes the step whatever
+// the scale.
+void scale_of(Attn& a, float score_scale) {
+    a.sl = fminf(fmaxf(score_scale * 1.44269504088896341f, 0x1p-149f), __FLT_MAX__);
+    a.step = fminf(8.f / a.sl, __FLT_MAX__);
+}
 
 constexpr int64_t MANY = 0x7fffffff;
 // what both attentions ask of their arguments
@@ -830,7 +832,7 @@ extern "C" int tcq_paged_attend(const void* q, int64_t q_tok, int64_t q_head, in
     a.table = table, a.cu = cu, a.lens = lens, a.o = (u16*)o;
     a.rows = rows, a.most = most, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.N = per_seq, a.shift = 31 - __builtin_clz(page_rows), a.pages = pages;
     a.cap = page_rows * per_seq, a.causal = causal != 0;
-    a.sl = log2_scale(score_scale);
+    scale_of(a, score_scale);
     return run(a, dtype == TCQ_BF16, true, B, min(keys, a.cap), part, (hipStream_t)stream);
 }
 
@@ -850,6 +852,6 @@ extern "C" int tcq_cross_attend(const void* q, int64_t q_tok, int64_t q_head, in
     a.kb = 2 * k_seq, a.kh = 2 * k_head, a.kt = 2 * k_tok, a.vb = 2 * v_seq, a.vh = 2 * v_head, a.vt = 2 * v_tok;
     a.mask = mask, a.mask_b = mask_seq, a.cu = cu, a.lens = lens, a.o = (u16*)o;
     a.rows = rows, a.most = most, a.Hk = Hk, a.G = Hq / Hk, a.D = D, a.cap = keys;
-    a.sl = log2_scale(score_scale);
+    scale_of(a, score_scale);
     return run(a, dtype == TCQ_BF16, false, B, keys, part, (hipStream_t)stream);
 }
