@@ -595,7 +595,7 @@ int tcq_gemmf_tcq_hT(const void* bits, const int8_t* t8, const void* hT, int ldh
  * Graph-capturable; what a call does follows from its inputs alone (pages are taken from the lowest free one on, for the sequences in order). All
  * calls on one bookkeeping belong on one stream, or on streams that wait for each other.
  *
- * tcq_pages_take: room for take[b] >= 0 more rows of every sequence: start[b] = lens[b], lens[b] += take[b]. A last page that is partly filled
+ * tcq_pages_take: room for take[b] >= 0 more rows of every sequence: start[b] (apart from lens and take) = lens[b], lens[b] += take[b]. A last page that is partly filled
  *   and held by other sequences too is replaced by a copy (k, v: the pools of all layers, (layers, pages) pages of page_bytes, a multiple of 16), if rows
  *   are taken; one that loses its last sequence so is free after the call. A sequence that lacks pages (those before it are served first) or entries
  *   stays as it is and adds one to lack. moves: 2 B + 1 ints of workspace.
@@ -606,7 +606,7 @@ int tcq_gemmf_tcq_hT(const void* bits, const int8_t* t8, const void* hT, int ldh
  *   moves: 2 pages + 2 ints of workspace.
  * tcq_pages_copy: page src[i] to page dst[i] in all layers, n pairs; pairs outside the pool are left out, no page may be a dst twice, or a dst and a
  *   src. The bookkeeping is not told.
- * tcq_paged_append: rows k, v (any strides in elements) to positions start[b] + i of their sequence: B equal shares of `most` rows, or rows cu[b] ..
+ * tcq_paged_append: rows k, v (any strides in elements; those of the pools such that no two of their rows overlap) to positions start[b] + i of their sequence: B equal shares of `most` rows, or rows cu[b] ..
  *   cu[b + 1] - 1, at most `most` of them. Rows at or past lens[b], and those whose entry names no page, are dropped. The
  *   pages that rows from the last take's start on go to are the sequence's own; others, and those forked since, change for all that hold them. */
 int tcq_pages_take(int32_t* table, int32_t* lens, int32_t* refs, int32_t* free, int32_t* lack, int B, int per_seq, int pages, int page_rows,
@@ -625,7 +625,7 @@ int tcq_paged_append(const void* k, int64_t k_tok, int64_t k_head, const void* v
 
 /* Softmax attention of q (rows, Hq, D), BF16 or FP16, D a multiple of 8 up to 256, over the first lens[b] rows of every sequence of such a cache (Hk
  * heads, Hq a multiple of Hk; q, k, v of one type; strides in elements, multiples of 8, a token's of at least D; 16-byte aligned): o (rows, Hq, D), contiguous. Rows of
- * sequence b: B equal shares of `most` rows, or rows cu[b] .. cu[b + 1] - 1, at most `most` of them. causal: row i of a sequence's n sees
+ * sequence b: B equal shares of `most` rows, or rows cu[b] .. cu[b + 1] - 1, at most `most` of them (none of some sequences, the last ones too). causal: row i of a sequence's n sees
  * positions up to lens[b] - n + i. A row that sees nothing is zeros; rows of no sequence are left as they are. An entry of the table outside the
  * pool counts as page 0. keys: about the longest length, for the split of the work alone. part: tcq_paged_attend_floats(...) floats of workspace
  * (0: none), 16-byte aligned, of this call alone. */

@@ -8,12 +8,15 @@
 // pieces whose place in the row is turned by the row's number so that the reads meet no bank twice.
 //
 // k_attend_rows, many rows: 32 rows a wave, so a wave reads every key and value of its tiles from LDS once for 32 rows: at 128 bytes a cycle that is as
-// long as its products (bound: LDS reads and vector instructions, 112 and 32 exponentials for 32 products a tile of 64 keys x 128 dims). 64
+// long as its products (bound: LDS reads and vector instructions, 144 and 32 exponentials for 32 products a tile of 64 keys x 128 dims). 64
 // rows a wave would halve the reads, but leave one wave a SIMD (297 us for the case below at 235 to 250), eight waves a workgroup share the writes
-// only (242), and scores of the next tile computed beside the exponentials of this one gain nothing while the reads bound both (260). MI355X:
-// 2 x 4096 rows of 16 heads x 128 to up to 4096 states 240 us (1000 TFLOP/s; an 8192^3 product reaches 1260), 256 dims 1060, 64 dims 890.
+// only (242), and scores of the next tile computed beside the exponentials of this one gain nothing while the reads bound both (260). (The times of that
+// comparison took the maximum off inside the exponentials' multiply-add, 1 to 2 % less, 64 dims 5.) MI355X, calls in a row: 2 x 4096 rows of 16 heads x 128
+// to up to 4096 states 236 to 246 us (980 to 1020 TFLOP/s; an 8192^3 product reaches 1260); to 4096 states, 8 heads x 256 1110 TFLOP/s, 32 x 64 880.
+// At 256 dims 2 to 12 registers spill over pages and with a mask (a mask that hides a fifth of those keys saves no time: 249 us after 247; 8 x 968 causal
+// rows of 8 heads on 1 x 256 in pages 65 us).
 // k_attend_few, few rows: 16 rows a workgroup, four waves that share the keys; bound by memory from some MB on: 32 sequences of 16 heads on 8 x 128
-// behind 4 to 8 thousand keys 149 us (814 MB, 5.5 TB/s), by latencies below (one row behind 968 keys 10.1 us with the join).
+// behind 4 to 8 thousand keys 149 us (814 MB, 5.5 TB/s), by latencies below (one row behind 968 keys 10.7 us with the join).
 #include "tcq_device.h"
 #include "tcq_launch.h"
 #include "tcq_paged_rows.h"

@@ -724,8 +724,8 @@ def _tables(what, table, lens):
 
 
 def paged_append(pages, k, v, table, lens, start, cu=None, most=None):
-    """Writes rows k, v (rows, H, D; the pages' type, any token and head strides) to positions start[b] .. of their sequence in the pages (one layer's) that
-    table (B, N) names, all int32 on the device: B equal shares of the rows, or rows cu[b] .. cu[b + 1] - 1 (most: at least the rows
+    """Writes rows k, v (rows, H, D; the pages' type, any token and head strides) to positions start[b] .. of their sequence in the pages (one layer's, any
+    strides whose rows do not overlap) that table (B, N) names, all int32 on the device: B equal shares of the rows, or rows cu[b] .. cu[b + 1] - 1 (most: at least the rows
     of any sequence). Rows at or past lens[b], the length with them, are dropped. What pages_take returns is start: it has made the pages that are
     written the sequence's own (rows before it, or ones that were forked since, may lie in pages that others hold, and change for all of them)."""
     ps, pk, pv, dt = _one_layer(pages, 'paged_append')
