@@ -56,3 +56,24 @@ def test_cross_attention_of_sequences_without_rows_last():
     q, k, v = rand(5, Hq, D, seed=1, by=2.0), rand(B, T, H, D, seed=2), rand(B, T, H, D, seed=3)
     got = K.cross_attend(q, k, v, cu=offsets(new), most=5)
     cross_check(got, q, k[:1], v[:1], [T], None, 5, BF)
+
+
+def test_prefill_chunks_of_sequences_in_turn():
+    """Parts of two prompts, behind each other and in turn, in a cache whose other sequences have no rows in a call, its capacity so long that the keys are split."""
+    from yanlongvla_amd import gemma, modules
+    model = gemma.make_policy(gemma.BackbonePolicy, DEV, seed=5, layers=2, vocab=512)
+    modules.install(model, runtime='fly', layers=gemma.synthetic_layers(model, 14, DEV))
+    prompts = [rand(n, 2048, seed=n) for n in (150, 97)]
+    sizes = [(64, 50, 36), (1, 64, 32)]
+    assert parts('tcq_paged_attend_floats', 50, 50, 4, 8, 1, 256, 600 * 16) > 1
+    with torch.inference_mode():
+        cache = gemma.PagedKVCache(2, 4, 600, 256, DEV, rows=16)
+        got = [[], []]
+        for i in range(3):
+            for b, (x, n) in enumerate(zip(prompts, sizes)):
+                at = sum(n[:i])
+                got[b].append(model.prefill_chunk(x[at:at + n[i]], cache, 2 * b))
+        assert cache.table.lens.tolist() == [150, 0, 97, 0] and cache.table.lack.item() == 0
+        for x, h in zip(prompts, got):
+            want = model.prefill(x)[0].float()
+            assert float((torch.cat(h).float() - want).norm() / want.norm()) < 0.03
